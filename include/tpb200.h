@@ -20,9 +20,9 @@
  *     (keepdim only changes the shape the caller reports, not the layout).
  *   - Every function returns TPB200_OK or an error code, never throws, never aborts;
  *     tpb200_last_error() gives the message of the calling thread's last failure.
- *   - Supported element type: float32 (TPB200_F32).  Other dtypes return
- *     TPB200_ERR_UNSUPPORTED so that an adapter can fall through to the kernel registered
- *     before it.
+ *   - Supported element type: float32 (TPB200_F32); the training operators also take bfloat16
+ *     and float16.  Other dtypes return TPB200_ERR_UNSUPPORTED so that an adapter can fall
+ *     through to the kernel registered before it.
  */
 #ifndef TPB200_H_
 #define TPB200_H_
@@ -47,6 +47,8 @@ extern "C" {
 
 /* dtypes */
 #define TPB200_F32 0
+#define TPB200_BF16 1   /* the training operators only */
+#define TPB200_F16 2    /* the training operators only */
 
 /* reduction operators.  The first eight replace, one to one, the kernels registered at
  * ReductionKernels.cu:386-391 and :410-417; the two fused forms serve callers that want
@@ -297,6 +299,107 @@ int tpb200_topk_merge(const float* cand_val, const int64_t* cand_idx, int64_t n_
 int tpb200_reduce_all_noalloc(int op, const void* in, int dtype, int64_t n, int64_t correction,
                               void* out_val, int64_t* out_idx, void* stream);
 
+/* ---- training operators -------------------------------------------------------------------------
+ * No reference counterpart.  Forward and backward of what a training step of a language model does to
+ * rows: objectives on logits, the residual path of a block, dropout.  Common to all of them:
+ *   - dtype is TPB200_F32, TPB200_BF16 or TPB200_F16; everything is computed in float32 or more, and
+ *     every output is rounded once.  Gradients have the type of what they are the gradient of.
+ *   - A tensor argument is [outer, inner, width] with unit stride along width: row (a, b) starts at
+ *     a * strides[0] + b * strides[1] elements (strides of 0 broadcast, any alignment is accepted).  A
+ *     value per token is a float32 (labels: int64) at a * strides[0] + b * strides[1].  Outputs are
+ *     contiguous and must not overlap an input.
+ *   - The results of a call do not depend on the order in which its CTAs run: no floating-point atomics.
+ *
+ * tpb200_token_logprobs: logp = logits[label] - lse, lse = log sum exp(logits), of every row.
+ * tpb200_token_logprobs_backward: grad_logits = grad_logp * ([j = label] - exp(logits - lse)).
+ *   A row with a negative label takes no part: it is not read, logp = lse = 0, its gradient is zero.  A
+ *   label of `vocab` or more gives NaN for its row (no access outside the row is made).  -inf logits have
+ *   probability 0; NaN, +inf and all -inf rows give NaN as log_softmax does.
+ */
+int tpb200_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t vocab,
+                          const int64_t* strides, const int64_t* labels, const int64_t* label_strides, float* logp,
+                          float* lse, void* stream);
+int tpb200_token_logprobs_backward(const float* grad_logp, const int64_t* grad_strides, const void* logits, int dtype,
+                                   int64_t outer, int64_t inner, int64_t vocab, const int64_t* strides,
+                                   const int64_t* labels, const int64_t* label_strides, const float* lse,
+                                   void* grad_logits, void* stream);
+
+/* Clipped policy loss with a KL term, and its gradient, in one call:
+ *   ratio = exp(logp - old_logp),  kl = exp(d) - d - 1 with d = ref_logp - logp
+ *   loss = sum over tokens of weight * (-min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coef kl)
+ *   grad_logits = grad_scale * d loss / d logits  (NULL: no gradient)
+ * weights carry the mask and the mean (1 / number of tokens, or per sequence); a token with a weight of
+ * zero or a negative label takes no part: its row is not read, its outputs and gradient are zero.
+ * ref_logp may be NULL with kl_coef = 0.  0 <= clip_low <= 1, clip_high >= 0, kl_coef >= 0.
+ */
+int tpb200_policy_loss(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t vocab, const int64_t* strides,
+                       const int64_t* labels, const int64_t* label_strides, const float* old_logp,
+                       const int64_t* old_strides, const float* advantages, const int64_t* advantage_strides,
+                       const float* weights, const int64_t* weight_strides, const float* ref_logp,
+                       const int64_t* ref_strides, double clip_low, double clip_high, double kl_coef, double grad_scale,
+                       float* loss, void* grad_logits, float* logp, float* ratio, float* kl, void* workspace,
+                       size_t workspace_bytes, void* stream);
+size_t tpb200_policy_loss_workspace_bytes(int64_t outer, int64_t inner);
+
+/* Preference loss on pairs of sequences, and its gradient.  Sequences 2 p and 2 p + 1 are the chosen and
+ * the rejected answer of pair p; sequence q is the rows offsets[q] .. offsets[q + 1] - 1 of packed logits
+ * (outer = 1; offsets: 2 * pairs + 1 non-decreasing int64 values in [0, inner] on the device), or, with
+ * offsets = NULL, the rows of outer index q (outer = 2 * pairs).
+ *   s_q = sum over the sequence of (logp - ref_logp),  rewards[q] = beta s_q,  m_p = rewards[2p] - rewards[2p+1]
+ *   loss = mean over pairs of -(1 - e) log sigmoid(m_p) - e log sigmoid(-m_p),  e = label_smoothing in [0, 0.5)
+ * Rows with a negative label and rows in no sequence take no part (their gradient is zero).  Offsets that
+ * decrease or leave [0, inner] are not followed: the loss is NaN.
+ */
+int tpb200_preference_loss(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t vocab,
+                           const int64_t* strides, const int64_t* labels, const int64_t* label_strides,
+                           const float* ref_logp, const int64_t* ref_strides, const int64_t* offsets, int64_t pairs,
+                           double beta, double label_smoothing, double grad_scale, float* loss, void* grad_logits,
+                           float* rewards, float* logp, void* workspace, size_t workspace_bytes, void* stream);
+size_t tpb200_preference_loss_workspace_bytes(int64_t outer, int64_t inner, int64_t pairs);
+
+/* Dropout from a counter-based generator (Philox 4x32-10): element i in row-major order is kept iff its 16
+ * bits of the block with counter (i / 8, offset) and key `seed` reach p in units of 2^-16 (rounded); kept
+ * elements are multiplied by 1 / (1 - p), with the p that was used, dropped ones are 0.  No mask is stored:
+ * the backward pass is the same call on the gradient.  0 <= p <= 1.
+ */
+int tpb200_dropout(const void* x, int dtype, int64_t outer, int64_t inner, int64_t width, const int64_t* strides,
+                   double p, uint64_t seed, uint64_t offset, void* y, void* stream);
+
+/* The residual path of a block: the norm after it, its gate, dropout and residual scale, and the norm
+ * before the next block, in one pass (hat(v) = v / sqrt(mean v^2 + eps)):
+ *   n = hat(h) * post_weight            (post_weight NULL: n = h, rstd_post is not written)
+ *   x_out = x + scale * gate * dropout(n)                                (gate NULL: 1)
+ *   y = hat(x_out) * next_weight        (next_weight NULL: no y, no rstd_next)
+ * y goes by x_out before it is rounded.  Rows of at most 16384 elements.
+ * The gate's kind, for the gradient: one row for all rows, one per outer index, or one for every row.
+ * The backward call gives the gradients of x, h, both weights and the gate from grad_x_out (NULL: zero)
+ * and grad_y; weight and gate gradients are sums over rows, taken in a fixed order.
+ * tpb200_rms_norm is y = hat(x) * weight alone.
+ */
+#define TPB200_GATE_NONE 0
+#define TPB200_GATE_VECTOR 1     /* [width]                    */
+#define TPB200_GATE_SEQUENCE 2   /* [outer, width]             */
+#define TPB200_GATE_ELEMENT 3    /* [outer, inner, width]      */
+int tpb200_block_residual(const void* x, const int64_t* x_strides, const void* h, const int64_t* h_strides, const void* gate,
+                          const int64_t* gate_strides, const void* post_weight, const void* next_weight, int dtype,
+                          int64_t outer, int64_t inner, int64_t width, double scale, double eps, double p, uint64_t seed,
+                          uint64_t offset, void* x_out, void* y, float* rstd_post, float* rstd_next, void* stream);
+int tpb200_block_residual_backward(const void* grad_x_out, const int64_t* grad_x_strides, const void* grad_y,
+                                   const int64_t* grad_y_strides, const void* h, const int64_t* h_strides, const void* x_out,
+                                   const int64_t* x_out_strides, const void* gate, const int64_t* gate_strides, int gate_kind,
+                                   const void* post_weight, const void* next_weight, const float* rstd_post,
+                                   const float* rstd_next, int dtype, int64_t outer, int64_t inner, int64_t width, double scale,
+                                   double p, uint64_t seed, uint64_t offset, void* grad_x, void* grad_h, void* grad_post,
+                                   void* grad_next, void* grad_gate, void* workspace, size_t workspace_bytes, void* stream);
+size_t tpb200_block_residual_backward_workspace_bytes(int64_t outer, int64_t inner, int64_t width, int has_post, int has_next,
+                                                      int gate_kind);
+int tpb200_rms_norm(const void* x, int dtype, int64_t outer, int64_t inner, int64_t width, const int64_t* strides,
+                    const void* weight, double eps, void* y, float* rstd, void* stream);
+int tpb200_rms_norm_backward(const void* grad_y, const int64_t* grad_strides, const void* x, const int64_t* strides, int dtype,
+                             int64_t outer, int64_t inner, int64_t width, const void* weight, const float* rstd, void* grad_x,
+                             void* grad_weight, void* workspace, size_t workspace_bytes, void* stream);
+size_t tpb200_rms_norm_backward_workspace_bytes(int64_t outer, int64_t inner, int64_t width);
+
 /* ---- diagnostics ------------------------------------------------------------------------------
  * Every device-side wait in these kernels is bounded: the ring and rendezvous waits between the
  * warps of a top-k CTA, and the wait of the fused exchange for the records of the other ranks.  A
@@ -319,7 +422,7 @@ int tpb200_device_status(int* status_out);
  *
  * tpb200_check_report fills info[0..5] = {1 in a checked build else 0, violations since the last
  * report, source file id of the first (1 reduce, 2 top-k, 3 top-k select, 4 softmax, 5 median,
- * 6 copy, 0 shared header), its line, its address, its size in bytes}, SYNCHRONISES and clears the
+ * 6 copy, 7 objectives on logits, 8 residual path, 9 dropout, 0 shared header), its line, its address, its size in bytes}, SYNCHRONISES and clears the
  * record.  tpb200_check_trim_next(bytes) is the checker's own test: the next entry point registers
  * every range `bytes` shorter at its end, so that correct kernels are seen to be caught and skipped;
  * TPB200_ERR_UNSUPPORTED in the ordinary build.  No reference counterpart.

@@ -18,7 +18,8 @@ LIB_PATH = os.path.join(_PKG, "libtpb200_checked.so" if CHECKED else ("libtpb200
 
 # error codes of include/tpb200.h
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_DIM_RANGE, ERR_EMPTY, ERR_WORKSPACE, ERR_CUDA = range(7)
-F32 = 0
+F32, BF16, F16 = 0, 1, 2
+GATE = {"none": 0, "vector": 1, "sequence": 2, "element": 3}
 OP = {"sum": 0, "mean": 1, "var": 2, "std": 3, "max": 4, "min": 5, "argmax": 6, "argmin": 7,
       "max_argmax": 8, "min_argmin": 9, "prod": 10, "norm1": 11, "norm2": 12, "norm_inf": 13,
       "norm_neg_inf": 14, "all": 15, "any": 16}
@@ -36,6 +37,10 @@ SYMBOLS = [
     "tpb200_comm_create", "tpb200_comm_destroy", "tpb200_comm_size", "tpb200_comm_fused", "tpb200_comm_stream",
     "tpb200_comm_synchronize", "tpb200_comm_result_values", "tpb200_comm_result_indices",
     "tpb200_reduce_sharded", "tpb200_topk_sharded", "tpb200_strided_copy",
+    "tpb200_token_logprobs", "tpb200_token_logprobs_backward", "tpb200_policy_loss", "tpb200_policy_loss_workspace_bytes",
+    "tpb200_preference_loss", "tpb200_preference_loss_workspace_bytes", "tpb200_dropout", "tpb200_block_residual",
+    "tpb200_block_residual_backward", "tpb200_block_residual_backward_workspace_bytes", "tpb200_rms_norm",
+    "tpb200_rms_norm_backward", "tpb200_rms_norm_backward_workspace_bytes",
 ]
 
 _I64P = ctypes.POINTER(ctypes.c_int64)
@@ -125,8 +130,45 @@ def lib() -> ctypes.CDLL:
     L.tpb200_topk_plan_info.argtypes = [i, i, _I64P, _I64P, i, i64, _I64P, i]
     L.tpb200_device_status.restype = i
     L.tpb200_device_status.argtypes = [ctypes.POINTER(ctypes.c_int)]
+    f64 = ctypes.c_double
+    logits, token = [vp, i, i64, i64, i64, _I64P], [vp, _I64P]     # rows of logits; a value per token
+    view = [vp, _I64P]                                              # [outer, inner, width] with two strides
+    L.tpb200_token_logprobs.restype = i
+    L.tpb200_token_logprobs.argtypes = [*logits, *token, vp, vp, vp]
+    L.tpb200_token_logprobs_backward.restype = i
+    L.tpb200_token_logprobs_backward.argtypes = [*token, *logits, *token, vp, vp, vp]
+    L.tpb200_policy_loss.restype = i
+    L.tpb200_policy_loss.argtypes = [*logits, *token * 5, f64, f64, f64, f64, vp, vp, vp, vp, vp, vp, sz, vp]
+    L.tpb200_policy_loss_workspace_bytes.restype = sz
+    L.tpb200_policy_loss_workspace_bytes.argtypes = [i64, i64]
+    L.tpb200_preference_loss.restype = i
+    L.tpb200_preference_loss.argtypes = [*logits, *token * 2, vp, i64, f64, f64, f64, vp, vp, vp, vp, vp, sz, vp]
+    L.tpb200_preference_loss_workspace_bytes.restype = sz
+    L.tpb200_preference_loss_workspace_bytes.argtypes = [i64, i64, i64]
+    L.tpb200_dropout.restype = i
+    L.tpb200_dropout.argtypes = [vp, i, i64, i64, i64, _I64P, f64, u64, u64, vp, vp]
+    L.tpb200_block_residual.restype = i
+    L.tpb200_block_residual.argtypes = [*view * 3, vp, vp, i, i64, i64, i64, f64, f64, f64, u64, u64, vp, vp, vp, vp, vp]
+    L.tpb200_block_residual_backward.restype = i
+    L.tpb200_block_residual_backward.argtypes = [*view * 5, i, vp, vp, vp, vp, i, i64, i64, i64, f64, f64, u64, u64, vp, vp, vp, vp, vp, vp, sz, vp]
+    L.tpb200_block_residual_backward_workspace_bytes.restype = sz
+    L.tpb200_block_residual_backward_workspace_bytes.argtypes = [i64, i64, i64, i, i, i]
+    L.tpb200_rms_norm.restype = i
+    L.tpb200_rms_norm.argtypes = [vp, i, i64, i64, i64, _I64P, vp, f64, vp, vp, vp]
+    L.tpb200_rms_norm_backward.restype = i
+    L.tpb200_rms_norm_backward.argtypes = [*view * 2, i, i64, i64, i64, vp, vp, vp, vp, vp, sz, vp]
+    L.tpb200_rms_norm_backward_workspace_bytes.restype = sz
+    L.tpb200_rms_norm_backward_workspace_bytes.argtypes = [i64, i64, i64]
     _lib = L
     return L
+
+
+_Pair = ctypes.c_int64 * 2
+
+
+def pair(a, b):
+    """Two int64 values (the strides of the rows of a training operator)."""
+    return _Pair(a, b)
 
 
 def i64_array(values):

@@ -21,7 +21,8 @@ LIB_PATH_CHECKED = os.path.join(_PKG, "libtpb200_checked.so")
 # and in the whole-tensor exchange, read by tensorplay_b200/trace.py.  A development build.
 LIB_PATH_TRACE = os.path.join(_PKG, "libtpb200_trace.so")
 
-SOURCES = ["api_common.cu", "reduce.cu", "topk.cu", "softmax.cu", "median.cu", "comm.cu", "copy.cu"]
+SOURCES = ["api_common.cu", "reduce.cu", "topk.cu", "softmax.cu", "median.cu", "comm.cu", "copy.cu",
+           "logprob.cu", "block_norm.cu", "dropout.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

@@ -1,0 +1,635 @@
+// The residual path of a block, forward and backward, behind tpb200_block_residual*, tpb200_rms_norm*.
+//
+// Forward, per row of `width` elements (hat(v) = v * rstd(v), rstd(v) = 1 / sqrt(mean v^2 + eps)):
+//     n = hat(h) * w_post                     the norm after the block (or n = h)
+//     x' = x + scale * gate * drop(n)         gate, dropout and residual scale
+//     y = hat(x') * w_next                    the norm before the next block (or no y)
+// Backward, from g_x = dL/dx' and g_y = dL/dy:
+//     a = g_y * w_next,  t = g_x + rstd_next * (a - hat(x') * mean(a * hat(x')))       = dL/dx
+//     d = scale * gate * factor * t,  dgate = scale * factor * n * t
+//     b = d * w_post,  dh = rstd_post * (b - hat(h) * mean(b * hat(h)))
+//     dw_next = sum over rows of g_y * hat(x'),  dw_post = sum over rows of d * hat(h)
+// rms_norm is the part with w_next alone.  All of it is float32 between the loads and the one rounding of
+// each output; y and rstd_next go by the x' before it is rounded.
+#define TPB_FILE_ID 8
+#include "host_util.h"
+#include "lowp.cuh"
+#include "philox.cuh"
+
+#include <algorithm>
+
+namespace tpb {
+
+constexpr int kMaxWidth = 16384;
+
+// Row (a, b) of a [outer, inner, width] view; strides of 0 broadcast.
+template <class T>
+struct RowView {
+    T* p;
+    long long s0, s1;
+    __device__ __forceinline__ T* row(long long a, long long b) const { return p + a * s0 + b * s1; }
+};
+
+template <class T>
+struct ForwardArgs {
+    RowView<const T> x, h, gate;     // h.p NULL: rms_norm alone; gate.p NULL: no gate
+    const T *post, *next;            // NULL: no such norm
+    T *x_out, *y;                    // contiguous
+    float *rstd_post, *rstd_next;
+    long long rows, inner;
+    int width;
+    float scale, eps;
+    DropSpec drop;
+};
+
+// Eight elements of a row per thread and step: consecutive ones (VEC: 16-byte vectors), or `nthr` apart.
+template <bool VEC>
+__device__ __forceinline__ int at(int u, int c, int tid, int nthr) {
+    return VEC ? (u * nthr + tid) * 8 + c : (u * 8 + c) * nthr + tid;
+}
+template <class T, bool VEC>
+__device__ __forceinline__ void fetch8(const T* p, int u, int tid, int nthr, int width, float* f) {
+    if (VEC) {
+        const int e = at<VEC>(u, 0, tid, nthr);
+        if (e < width) load8(p + e, f);
+        else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) f[c] = 0.0f;
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const int e = at<VEC>(u, c, tid, nthr);
+            f[c] = e < width ? Elem<T>::get(*TPB_CK(&p[e])) : 0.0f;
+        }
+    }
+}
+template <class T, bool VEC>
+__device__ __forceinline__ void put8(T* p, int u, int tid, int nthr, int width, const float* f) {
+    if (VEC) {
+        const int e = at<VEC>(u, 0, tid, nthr);
+        if (e < width) store8(p + e, f);
+    } else {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const int e = at<VEC>(u, c, tid, nthr);
+            if (e < width) *TPB_CK(&p[e]) = Elem<T>::put(f[c]);
+        }
+    }
+}
+template <bool VEC>
+__device__ __forceinline__ void factors8(const DropSpec& d, long long r, int u, int tid, int nthr, int width, float* f) {
+    if (d.units == 0) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) f[c] = 1.0f;
+    } else if (VEC) {
+        drop_factors8((unsigned long long)(r * (width >> 3) + (u * nthr + tid)), d, f);
+    } else {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) f[c] = drop_factor1((unsigned long long)(r * width + at<VEC>(u, c, tid, nthr)), d);
+    }
+}
+
+// Sum over the threads of a row: a warp, or the CTA (`red` then has 32 slots that the next call must not reuse).
+template <bool WARP>
+__device__ __forceinline__ float row_add(float v, float* red) {
+    v = warp_add(v);
+    if (WARP) return v;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    if (lane == 0) red[warp] = v;
+    __syncthreads();
+    return warp_add(lane < nw ? red[lane] : 0.0f);
+}
+
+template <class T, int NV, bool VEC, bool WARP>
+__global__ void __launch_bounds__(1024)
+block_forward_kernel(ForwardArgs<T> k) {
+    __shared__ float red[2][32];
+    const int tid = WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x, nthr = WARP ? 32 : (int)blockDim.x;
+    const long long r = WARP ? (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : (long long)blockIdx.x;
+    if (WARP && r >= k.rows) return;
+    const long long a = r / k.inner, b = r - a * k.inner;
+    const float inv_width = 1.0f / (float)k.width;
+    float x[NV][8], h[NV][8];
+    const T* px = k.x.row(a, b);
+#pragma unroll
+    for (int u = 0; u < NV; ++u) fetch8<T, VEC>(px, u, tid, nthr, k.width, x[u]);
+    if (k.h.p) {
+        const T* ph = k.h.row(a, b);
+#pragma unroll
+        for (int u = 0; u < NV; ++u) fetch8<T, VEC>(ph, u, tid, nthr, k.width, h[u]);
+        float rstd = 1.0f;
+        if (k.post) {
+            float s = 0.0f;
+#pragma unroll
+            for (int u = 0; u < NV; ++u)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) s = fmaf(h[u][c], h[u][c], s);
+            rstd = rsqrtf(row_add<WARP>(s, red[0]) * inv_width + k.eps);
+            if (tid == 0) *TPB_CK(&k.rstd_post[r]) = rstd;
+        }
+        const T* pg = k.gate.p ? k.gate.row(a, b) : nullptr;
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            float w[8], f[8];
+            if (k.post) {
+                fetch8<T, VEC>(k.post, u, tid, nthr, k.width, w);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) h[u][c] = h[u][c] * rstd * w[c];
+            }
+            if (k.drop.units) {
+                factors8<VEC>(k.drop, r, u, tid, nthr, k.width, f);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) h[u][c] = f[c] == 0.0f ? 0.0f : h[u][c] * f[c];
+            }
+            if (pg) {
+                fetch8<T, VEC>(pg, u, tid, nthr, k.width, w);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) h[u][c] *= w[c];
+            }
+#pragma unroll
+            for (int c = 0; c < 8; ++c) x[u][c] = fmaf(k.scale, h[u][c], x[u][c]);
+            put8<T, VEC>(k.x_out + r * k.width, u, tid, nthr, k.width, x[u]);
+        }
+    }
+    if (!k.next) return;
+    float s = 0.0f;
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) s = fmaf(x[u][c], x[u][c], s);   // elements past the width are zero
+    const float rstd = rsqrtf(row_add<WARP>(s, red[1]) * inv_width + k.eps);
+    if (tid == 0) *TPB_CK(&k.rstd_next[r]) = rstd;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        float w[8];
+        fetch8<T, VEC>(k.next, u, tid, nthr, k.width, w);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) w[c] *= x[u][c] * rstd;
+        put8<T, VEC>(k.y + r * k.width, u, tid, nthr, k.width, w);
+    }
+}
+
+template <class T>
+struct BackwardArgs {
+    RowView<const T> grad_x, grad_y, h, x_out, gate;   // grad_x.p NULL: zero; grad_y.p / x_out.p go with next
+    const T *post, *next;
+    const float *rstd_post, *rstd_next;
+    T *dx, *dh, *dgate;                // contiguous; dgate: [groups, width], or all rows (gate_rows)
+    float *part_post, *part_next, *part_gate;   // [workers, width] sums over a worker's rows
+    long long rows, inner;
+    // worker k takes the rows [lo, hi) of split k % splits of group k / splits (group_len rows each,
+    // split_len rows per split), or, with groups_per_worker > 0, that many whole groups
+    long long group_len, split_len, groups_per_worker;
+    int splits, workers, width;
+    int gate_rows;                     // 1: the gate has a row for every row
+    float scale;
+    DropSpec drop;
+};
+
+template <class T, int NV, bool VEC, bool WARP>
+__global__ void __launch_bounds__(1024)
+block_backward_kernel(BackwardArgs<T> k) {
+    __shared__ float red[2][32];
+    const int tid = WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x, nthr = WARP ? 32 : (int)blockDim.x;
+    const int worker = WARP ? (int)(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) : (int)blockIdx.x;
+    if (WARP && worker >= k.workers) return;
+    const float inv_width = 1.0f / (float)k.width;
+    long long lo, hi;
+    if (k.groups_per_worker > 0) {
+        lo = (long long)worker * k.groups_per_worker * k.group_len;
+        hi = lo + k.groups_per_worker * k.group_len;
+        if (hi > k.rows) hi = k.rows;
+    } else {
+        const long long g = worker / k.splits, s = worker - g * k.splits;
+        lo = s * k.split_len;
+        hi = lo + k.split_len;
+        if (hi > k.group_len) hi = k.group_len;
+        lo += g * k.group_len;
+        hi += g * k.group_len;
+    }
+    const bool sum_gate = k.gate.p && !k.gate_rows;
+    float acc_post[NV][8], acc_next[NV][8], acc_gate[NV][8];
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) acc_post[u][c] = acc_next[u][c] = acc_gate[u][c] = 0.0f;
+    for (long long r = lo; r < hi; ++r) {
+        const long long a = r / k.inner, b = r - a * k.inner;
+        float t[NV][8], h[NV][8];
+        if (k.grad_x.p) {
+#pragma unroll
+            for (int u = 0; u < NV; ++u) fetch8<T, VEC>(k.grad_x.row(a, b), u, tid, nthr, k.width, t[u]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < NV; ++u)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) t[u][c] = 0.0f;
+        }
+        if (k.h.p) {
+#pragma unroll
+            for (int u = 0; u < NV; ++u) fetch8<T, VEC>(k.h.row(a, b), u, tid, nthr, k.width, h[u]);
+        }
+        if (k.next) {
+            const float rstd = *TPB_CK(&k.rstd_next[r]);
+            float xh[NV][8], g[NV][8], s = 0.0f;
+#pragma unroll
+            for (int u = 0; u < NV; ++u) {
+                float w[8];
+                fetch8<T, VEC>(k.x_out.row(a, b), u, tid, nthr, k.width, xh[u]);
+                fetch8<T, VEC>(k.grad_y.row(a, b), u, tid, nthr, k.width, g[u]);
+                fetch8<T, VEC>(k.next, u, tid, nthr, k.width, w);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    xh[u][c] *= rstd;
+                    acc_next[u][c] = fmaf(g[u][c], xh[u][c], acc_next[u][c]);
+                    g[u][c] *= w[c];
+                    s = fmaf(g[u][c], xh[u][c], s);
+                }
+            }
+            const float m = row_add<WARP>(s, red[0]) * inv_width;
+#pragma unroll
+            for (int u = 0; u < NV; ++u)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) t[u][c] = fmaf(rstd, g[u][c] - xh[u][c] * m, t[u][c]);
+        }
+#pragma unroll
+        for (int u = 0; u < NV; ++u) put8<T, VEC>(k.dx + r * k.width, u, tid, nthr, k.width, t[u]);
+        if (k.h.p) {
+            const float rstd = k.post ? *TPB_CK(&k.rstd_post[r]) : 1.0f;
+            float s = 0.0f;
+#pragma unroll
+            for (int u = 0; u < NV; ++u) {
+                float w[8], f[8], g[8];
+                if (k.post) fetch8<T, VEC>(k.post, u, tid, nthr, k.width, w);
+                factors8<VEC>(k.drop, r, u, tid, nthr, k.width, f);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    h[u][c] *= rstd;
+                    f[c] *= k.scale;
+                    t[u][c] *= f[c];                                   // scale * factor * t
+                }
+                if (k.gate.p) {
+                    fetch8<T, VEC>(k.gate.row(a, b), u, tid, nthr, k.width, g);
+                    float dg[8];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const float n = k.post ? h[u][c] * w[c] : h[u][c];
+                        dg[c] = f[c] == 0.0f ? 0.0f : n * t[u][c];
+                        acc_gate[u][c] += dg[c];
+                        t[u][c] *= g[c];
+                    }
+                    if (k.gate_rows) put8<T, VEC>(k.dgate + r * k.width, u, tid, nthr, k.width, dg);
+                }
+                if (k.post) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        acc_post[u][c] = fmaf(t[u][c], h[u][c], acc_post[u][c]);
+                        t[u][c] *= w[c];
+                        s = fmaf(t[u][c], h[u][c], s);
+                    }
+                }
+            }
+            if (k.post) {
+                const float m = row_add<WARP>(s, red[1]) * inv_width;
+#pragma unroll
+                for (int u = 0; u < NV; ++u)
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) t[u][c] = rstd * (t[u][c] - h[u][c] * m);
+            }
+#pragma unroll
+            for (int u = 0; u < NV; ++u) put8<T, VEC>(k.dh + r * k.width, u, tid, nthr, k.width, t[u]);
+            if (sum_gate && k.groups_per_worker > 0 && (r + 1) % k.group_len == 0) {   // the group is complete
+                const long long g = r / k.group_len;
+#pragma unroll
+                for (int u = 0; u < NV; ++u) {
+                    put8<T, VEC>(k.dgate + g * k.width, u, tid, nthr, k.width, acc_gate[u]);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) acc_gate[u][c] = 0.0f;
+                }
+            }
+        }
+        if (!WARP) __syncthreads();   // the slots of row_add are free again
+    }
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        if (k.post && k.h.p) put8<float, VEC>(k.part_post + (long long)worker * k.width, u, tid, nthr, k.width, acc_post[u]);
+        if (k.next) put8<float, VEC>(k.part_next + (long long)worker * k.width, u, tid, nthr, k.width, acc_next[u]);
+        if (sum_gate && k.groups_per_worker == 0) put8<float, VEC>(k.part_gate + (long long)worker * k.width, u, tid, nthr, k.width, acc_gate[u]);
+    }
+}
+
+// Column sums of the workers' partial sums in a fixed order: 32 columns by 8 slots at a time.
+// blockIdx.y: 0 w_post, 1 w_next, 2 + g the gate's group g (slots g * splits ...).
+template <class T>
+__global__ void __launch_bounds__(256)
+block_sums_kernel(const float* __restrict__ part_post, const float* __restrict__ part_next, const float* __restrict__ part_gate,
+                  T* __restrict__ dpost, T* __restrict__ dnext, T* __restrict__ dgate, int workers, int splits, int width) {
+    __shared__ double red[8][33];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), y = threadIdx.x >> 5;
+    const int what = (int)blockIdx.y;
+    const float* src = what == 0 ? part_post : (what == 1 ? part_next : part_gate + (long long)(what - 2) * splits * width);
+    T* dst = what == 0 ? dpost : (what == 1 ? dnext : dgate + (long long)(what - 2) * width);
+    if (!src || !dst) return;
+    const int n = what < 2 ? workers : splits;
+    double s = 0.0;
+    if (c < width)
+        for (int i = y; i < n; i += 8) s += (double)*TPB_CK(&src[(long long)i * width + c]);
+    red[y][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (y == 0 && c < width) {
+        s = 0.0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += red[j][threadIdx.x & 31];
+        *TPB_CK(&dst[c]) = Elem<T>::put((float)s);
+    }
+}
+
+// ---------------------------------------------------------------- host side -------------------
+struct RowPlan {
+    bool vec, warp;
+    int nv, threads;   // threads of a CTA
+};
+inline RowPlan plan_rows(int64_t width, bool vec) {
+    RowPlan p;
+    p.vec = vec;
+    p.warp = width <= 512;
+    p.nv = width <= 256 || (width > 512 && width <= 8192) ? 1 : 2;
+    p.threads = p.warp ? 256 : (int)std::min<long long>(1024, round_up(ceil_div(width, 8 * p.nv), 32));
+    return p;
+}
+
+// How the rows are shared out for the backward pass; depends on sizes only, for the workspace query.
+struct Sharing {
+    long long groups, group_len, split_len, groups_per_worker;
+    int splits, workers;
+};
+inline Sharing share_rows(long long rows, long long groups, int64_t width) {
+    const RowPlan p = plan_rows(width, true);
+    const long long most = p.warp ? 8LL * 4 * sm_count() : (long long)sm_count() * std::max(1, 1024 / p.threads);
+    Sharing s{groups, rows / groups, 0, 0, 1, 1};
+    if (groups > 1 && groups >= most) {
+        s.groups_per_worker = ceil_div(groups, most);
+        s.workers = (int)ceil_div(groups, s.groups_per_worker);
+        return s;
+    }
+    const long long want = std::max(1LL, std::min(most / groups, s.group_len));
+    s.split_len = ceil_div(s.group_len, want);
+    s.splits = (int)ceil_div(s.group_len, s.split_len);
+    s.workers = (int)(groups * s.splits);
+    return s;
+}
+
+template <class T, class K>
+bool aligned_row(const RowView<K>& v) { return (((uintptr_t)v.p) & 15) == 0 && (v.s0 * (long long)sizeof(T)) % 16 == 0 && (v.s1 * (long long)sizeof(T)) % 16 == 0; }
+inline bool aligned16(const void* p) { return (((uintptr_t)p) & 15) == 0; }
+
+#define TPB_BLOCK_LAUNCH(KERNEL, T, plan, grid, st, args)                                                                       \
+    do {                                                                                                                         \
+        if ((plan).warp) {                                                                                                       \
+            if ((plan).vec) { if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, true, true>), grid, (plan).threads, 0, st, args);    \
+                              else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, true, true>), grid, (plan).threads, 0, st, args); }           \
+            else            { if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, false, true>), grid, (plan).threads, 0, st, args);   \
+                              else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, false, true>), grid, (plan).threads, 0, st, args); }          \
+        } else {                                                                                                                 \
+            if ((plan).vec) { if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, true, false>), grid, (plan).threads, 0, st, args);   \
+                              else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, true, false>), grid, (plan).threads, 0, st, args); }          \
+            else            { if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, false, false>), grid, (plan).threads, 0, st, args);  \
+                              else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, false, false>), grid, (plan).threads, 0, st, args); }         \
+        }                                                                                                                        \
+    } while (0)
+
+template <class T>
+int forward_run(const ForwardArgs<T>& k, cudaStream_t st) {
+    const bool vec = k.width % 8 == 0 && aligned_row<T>(k.x) && (!k.h.p || aligned_row<T>(k.h)) && (!k.gate.p || aligned_row<T>(k.gate)) &&
+                     aligned16(k.post) && aligned16(k.next) && aligned16(k.x_out) && aligned16(k.y);
+    const RowPlan p = plan_rows(k.width, vec);
+    const dim3 grid((unsigned)(p.warp ? ceil_div(k.rows, p.threads / 32) : k.rows));
+    TPB_BLOCK_LAUNCH(block_forward_kernel, T, p, grid, st, k);
+    return TPB200_OK;
+}
+
+template <class T>
+int backward_run(const BackwardArgs<T>& k, T* dpost, T* dnext, long long gate_groups, cudaStream_t st) {
+    const bool vec = k.width % 8 == 0 && (!k.grad_x.p || aligned_row<T>(k.grad_x)) && (!k.grad_y.p || aligned_row<T>(k.grad_y)) &&
+                     (!k.h.p || aligned_row<T>(k.h)) && (!k.x_out.p || aligned_row<T>(k.x_out)) && (!k.gate.p || aligned_row<T>(k.gate)) &&
+                     aligned16(k.post) && aligned16(k.next) && aligned16(k.dx) && aligned16(k.dh) && aligned16(k.dgate);
+    RowPlan p = plan_rows(k.width, vec);
+    const dim3 grid((unsigned)(p.warp ? ceil_div(k.workers, p.threads / 32) : k.workers));
+    TPB_BLOCK_LAUNCH(block_backward_kernel, T, p, grid, st, k);
+    const bool sum_gate = k.gate.p && !k.gate_rows && k.groups_per_worker == 0;
+    if (!dpost && !dnext && !sum_gate) return TPB200_OK;
+    const dim3 sums((unsigned)ceil_div(k.width, 32), (unsigned)(2 + (sum_gate ? gate_groups : 0)));
+    TPB_LAUNCH("block_sums_kernel", block_sums_kernel<T>, sums, 256, 0, st, (const float*)k.part_post, (const float*)k.part_next,
+               (const float*)k.part_gate, dpost, dnext, sum_gate ? k.dgate : (T*)nullptr, k.workers, k.splits, k.width);
+    return TPB200_OK;
+}
+
+template <class T>
+RowView<const T> view_of(const void* p, const int64_t* s) {
+    return RowView<const T>{(const T*)p, p && s ? s[0] : 0, p && s ? s[1] : 0};
+}
+
+int check_block(const char* what, int dtype, int64_t outer, int64_t inner, int64_t width) {
+    TPB_TRY_ROWS(what, dtype, outer, inner, width);
+    if (width > kMaxWidth) return fail(TPB200_ERR_UNSUPPORTED, "%s: rows of at most %d elements (got %lld)", what, kMaxWidth, (long long)width);
+    return TPB200_OK;
+}
+
+// groups of rows that share a row of the gate, by the gate's kind; 0: an unknown kind
+inline long long gate_groups_of(int kind, int64_t outer) { return kind == TPB200_GATE_SEQUENCE ? outer : 1; }
+
+struct BlockPointers { float *post, *next, *gate; size_t bytes; };
+inline BlockPointers block_workspace(void* ws, const Sharing& s, int64_t width, bool post, bool next, bool gate) {
+    BlockPointers b{nullptr, nullptr, nullptr, 0};
+    const size_t each = (size_t)round_up((long long)s.workers * width * 4, 256);
+    if (post) { b.post = (float*)((char*)ws + b.bytes); b.bytes += each; }
+    if (next) { b.next = (float*)((char*)ws + b.bytes); b.bytes += each; }
+    if (gate && s.groups_per_worker == 0) { b.gate = (float*)((char*)ws + b.bytes); b.bytes += each; }
+    return b;
+}
+
+template <class T>
+int forward_call(const void* x, const int64_t* xs, const void* h, const int64_t* hs, const void* gate, const int64_t* gs, const void* post,
+                 const void* next, int64_t outer, int64_t inner, int64_t width, double scale, double eps, const DropSpec& drop, void* x_out,
+                 void* y, float* rstd_post, float* rstd_next, cudaStream_t st) {
+    ForwardArgs<T> k{};
+    k.x = view_of<T>(x, xs);
+    k.h = view_of<T>(h, hs);
+    k.gate = view_of<T>(gate, gs);
+    k.post = (const T*)post;
+    k.next = (const T*)next;
+    k.x_out = (T*)x_out;
+    k.y = (T*)y;
+    k.rstd_post = rstd_post;
+    k.rstd_next = rstd_next;
+    k.rows = outer * inner;
+    k.inner = inner;
+    k.width = (int)width;
+    k.scale = (float)scale;
+    k.eps = (float)eps;
+    k.drop = drop;
+    return forward_run<T>(k, st);
+}
+
+struct BackwardCall {
+    const void *grad_x, *grad_y, *h, *x_out, *gate, *post, *next;
+    const int64_t *gxs, *gys, *hs, *xs, *gs;
+    const float *rstd_post, *rstd_next;
+    void *dx, *dh, *dgate, *dpost, *dnext;
+    int64_t outer, inner, width;
+    int gate_kind;
+    double scale;
+    DropSpec drop;
+    Sharing share;
+    BlockPointers ws;
+};
+template <class T>
+int backward_call(const BackwardCall& c, cudaStream_t st) {
+    BackwardArgs<T> k{};
+    k.grad_x = view_of<T>(c.grad_x, c.gxs);
+    k.grad_y = view_of<T>(c.grad_y, c.gys);
+    k.h = view_of<T>(c.h, c.hs);
+    k.x_out = view_of<T>(c.x_out, c.xs);
+    k.gate = view_of<T>(c.gate, c.gs);
+    k.post = (const T*)c.post;
+    k.next = (const T*)c.next;
+    k.rstd_post = c.rstd_post;
+    k.rstd_next = c.rstd_next;
+    k.dx = (T*)c.dx;
+    k.dh = (T*)c.dh;
+    k.dgate = (T*)c.dgate;
+    k.part_post = c.ws.post;
+    k.part_next = c.ws.next;
+    k.part_gate = c.ws.gate;
+    k.rows = c.outer * c.inner;
+    k.inner = c.inner;
+    k.group_len = c.share.group_len;
+    k.split_len = c.share.split_len;
+    k.groups_per_worker = c.share.groups_per_worker;
+    k.splits = c.share.splits;
+    k.workers = c.share.workers;
+    k.width = (int)c.width;
+    k.gate_rows = c.gate_kind == TPB200_GATE_ELEMENT;
+    k.scale = (float)c.scale;
+    k.drop = c.drop;
+    return backward_run<T>(k, (T*)c.dpost, (T*)c.dnext, c.share.groups, st);
+}
+
+}  // namespace tpb
+
+using namespace tpb;
+
+extern "C" int tpb200_rms_norm(const void* x, int dtype, int64_t outer, int64_t inner, int64_t width, const int64_t* strides,
+                               const void* weight, double eps, void* y, float* rstd, void* stream) {
+    const int rc = check_block("rms_norm", dtype, outer, inner, width);
+    if (rc != TPB200_OK) return rc;
+    if (!(eps >= 0.0)) return fail(TPB200_ERR_INVALID, "rms_norm: eps must not be negative");
+    if (outer * inner * width == 0) return TPB200_OK;
+    if (!x || !strides || !weight || !y || !rstd) return fail(TPB200_ERR_INVALID, "rms_norm: NULL pointer argument");
+    cudaStream_t st = (cudaStream_t)stream;
+    const int64_t e = dtype_bytes(dtype), n = outer * inner;
+    TPB_CHECK_RANGES(st, rows_range(x, outer, inner, width, strides, e), HostRange{weight, (size_t)(width * e)}, HostRange{y, (size_t)(n * width * e)},
+                     HostRange{rstd, (size_t)n * 4});
+    const DropSpec none{0, 0, 0, 1.0f};
+    if (dtype == TPB200_F32) return forward_call<float>(x, strides, nullptr, nullptr, nullptr, nullptr, nullptr, weight, outer, inner, width, 1.0, eps, none, nullptr, y, nullptr, rstd, st);
+    if (dtype == TPB200_BF16) return forward_call<__nv_bfloat16>(x, strides, nullptr, nullptr, nullptr, nullptr, nullptr, weight, outer, inner, width, 1.0, eps, none, nullptr, y, nullptr, rstd, st);
+    return forward_call<__half>(x, strides, nullptr, nullptr, nullptr, nullptr, nullptr, weight, outer, inner, width, 1.0, eps, none, nullptr, y, nullptr, rstd, st);
+}
+
+extern "C" int tpb200_block_residual(const void* x, const int64_t* x_strides, const void* h, const int64_t* h_strides, const void* gate,
+                                     const int64_t* gate_strides, const void* post_weight, const void* next_weight, int dtype,
+                                     int64_t outer, int64_t inner, int64_t width, double scale, double eps, double p, uint64_t seed,
+                                     uint64_t offset, void* x_out, void* y, float* rstd_post, float* rstd_next, void* stream) {
+    const int rc = check_block("block_residual", dtype, outer, inner, width);
+    if (rc != TPB200_OK) return rc;
+    if (!(eps >= 0.0)) return fail(TPB200_ERR_INVALID, "block_residual: eps must not be negative");
+    DropSpec drop;
+    if (!make_drop(p, seed, offset, &drop)) return fail(TPB200_ERR_INVALID, "block_residual: p must lie in [0, 1]");
+    if (outer * inner * width == 0) return TPB200_OK;
+    if (!x || !h || !x_out || !x_strides || !h_strides || (gate && !gate_strides) || (post_weight && !rstd_post) || (next_weight && (!y || !rstd_next)))
+        return fail(TPB200_ERR_INVALID, "block_residual: NULL pointer argument");
+    cudaStream_t st = (cudaStream_t)stream;
+    const int64_t e = dtype_bytes(dtype), n = outer * inner;
+    TPB_CHECK_RANGES(st, rows_range(x, outer, inner, width, x_strides, e), rows_range(h, outer, inner, width, h_strides, e),
+                     rows_range(gate, outer, inner, width, gate_strides, e), HostRange{post_weight, (size_t)(width * e)},
+                     HostRange{next_weight, (size_t)(width * e)}, HostRange{x_out, (size_t)(n * width * e)}, HostRange{y, y ? (size_t)(n * width * e) : 0},
+                     HostRange{rstd_post, (size_t)n * 4}, HostRange{rstd_next, (size_t)n * 4});
+    if (dtype == TPB200_F32) return forward_call<float>(x, x_strides, h, h_strides, gate, gate_strides, post_weight, next_weight, outer, inner, width, scale, eps, drop, x_out, y, rstd_post, rstd_next, st);
+    if (dtype == TPB200_BF16) return forward_call<__nv_bfloat16>(x, x_strides, h, h_strides, gate, gate_strides, post_weight, next_weight, outer, inner, width, scale, eps, drop, x_out, y, rstd_post, rstd_next, st);
+    return forward_call<__half>(x, x_strides, h, h_strides, gate, gate_strides, post_weight, next_weight, outer, inner, width, scale, eps, drop, x_out, y, rstd_post, rstd_next, st);
+}
+
+extern "C" size_t tpb200_block_residual_backward_workspace_bytes(int64_t outer, int64_t inner, int64_t width, int has_post, int has_next,
+                                                                 int gate_kind) {
+    if (outer <= 0 || inner <= 0 || width <= 0 || outer > 0x7fffffffLL || inner > 0x7fffffffLL || outer * inner > 0x7fffffffLL || width > kMaxWidth) return 0;
+    const Sharing s = share_rows(outer * inner, gate_groups_of(gate_kind, outer), width);
+    return block_workspace(nullptr, s, width, has_post != 0, has_next != 0, gate_kind == TPB200_GATE_VECTOR || gate_kind == TPB200_GATE_SEQUENCE).bytes;
+}
+
+extern "C" int tpb200_block_residual_backward(const void* grad_x_out, const int64_t* grad_x_strides, const void* grad_y,
+                                              const int64_t* grad_y_strides, const void* h, const int64_t* h_strides, const void* x_out,
+                                              const int64_t* x_out_strides, const void* gate, const int64_t* gate_strides, int gate_kind,
+                                              const void* post_weight, const void* next_weight, const float* rstd_post,
+                                              const float* rstd_next, int dtype, int64_t outer, int64_t inner, int64_t width, double scale,
+                                              double p, uint64_t seed, uint64_t offset, void* grad_x, void* grad_h, void* grad_post,
+                                              void* grad_next, void* grad_gate, void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = check_block("block_residual_backward", dtype, outer, inner, width);
+    if (rc != TPB200_OK) return rc;
+    if (gate_kind < TPB200_GATE_NONE || gate_kind > TPB200_GATE_ELEMENT) return fail(TPB200_ERR_INVALID, "block_residual_backward: unknown gate kind %d", gate_kind);
+    BackwardCall c{};
+    if (!make_drop(p, seed, offset, &c.drop)) return fail(TPB200_ERR_INVALID, "block_residual_backward: p must lie in [0, 1]");
+    const int64_t n = outer * inner, e = dtype_bytes(dtype);
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool gated = gate_kind != TPB200_GATE_NONE && h;
+    if (n * width == 0) {   // sums over no rows are zero
+        if (width > 0 && post_weight && grad_post) TPB_CUDA_OK(cudaMemsetAsync(grad_post, 0, (size_t)(width * e), st));
+        if (width > 0 && next_weight && grad_next) TPB_CUDA_OK(cudaMemsetAsync(grad_next, 0, (size_t)(width * e), st));
+        if (width > 0 && grad_gate && gate_kind == TPB200_GATE_VECTOR) TPB_CUDA_OK(cudaMemsetAsync(grad_gate, 0, (size_t)(width * e), st));
+        if (width > 0 && grad_gate && gate_kind == TPB200_GATE_SEQUENCE && outer > 0) TPB_CUDA_OK(cudaMemsetAsync(grad_gate, 0, (size_t)(outer * width * e), st));
+        return TPB200_OK;
+    }
+    if (!grad_x || (grad_x_out && !grad_x_strides) || (next_weight && (!grad_y || !grad_y_strides || !x_out || !x_out_strides || !rstd_next || !grad_next)) ||
+        (h && (!h_strides || !grad_h)) || (h && post_weight && (!rstd_post || !grad_post)) || (gated && (!gate || !gate_strides || !grad_gate)))
+        return fail(TPB200_ERR_INVALID, "block_residual_backward: NULL pointer argument");
+    c.share = share_rows(n, gated ? gate_groups_of(gate_kind, outer) : 1, width);
+    c.ws = block_workspace(workspace, c.share, width, h && post_weight, next_weight != nullptr, gated && gate_kind != TPB200_GATE_ELEMENT);
+    if (c.ws.bytes > 0 && (!workspace || workspace_bytes < c.ws.bytes))
+        return fail(TPB200_ERR_WORKSPACE, "block_residual_backward: workspace missing or too small (%zu of %zu bytes)", workspace_bytes, c.ws.bytes);
+    c.grad_x = grad_x_out; c.gxs = grad_x_strides;
+    c.grad_y = next_weight ? grad_y : nullptr; c.gys = grad_y_strides;
+    c.h = h; c.hs = h_strides;
+    c.x_out = next_weight ? x_out : nullptr; c.xs = x_out_strides;
+    c.gate = gated ? gate : nullptr; c.gs = gate_strides;
+    c.post = h ? post_weight : nullptr; c.next = next_weight;
+    c.rstd_post = rstd_post; c.rstd_next = rstd_next;
+    c.dx = grad_x; c.dh = grad_h; c.dgate = gated ? grad_gate : nullptr;
+    c.dpost = c.post ? grad_post : nullptr; c.dnext = next_weight ? grad_next : nullptr;
+    c.outer = outer; c.inner = inner; c.width = width;
+    c.gate_kind = gated ? gate_kind : TPB200_GATE_NONE;
+    c.scale = scale;
+    const int64_t gate_rows = gate_kind == TPB200_GATE_ELEMENT ? n : gate_groups_of(gate_kind, outer);
+    TPB_CHECK_RANGES(st, rows_range(c.grad_x, outer, inner, width, grad_x_strides, e), rows_range(c.grad_y, outer, inner, width, grad_y_strides, e),
+                     rows_range(h, outer, inner, width, h_strides, e), rows_range(c.x_out, outer, inner, width, x_out_strides, e),
+                     rows_range(c.gate, outer, inner, width, gate_strides, e), HostRange{post_weight, (size_t)(width * e)},
+                     HostRange{next_weight, (size_t)(width * e)}, HostRange{rstd_post, (size_t)n * 4}, HostRange{rstd_next, (size_t)n * 4},
+                     HostRange{grad_x, (size_t)(n * width * e)}, HostRange{c.h ? grad_h : nullptr, (size_t)(n * width * e)},
+                     HostRange{c.dgate, (size_t)(gate_rows * width * e)}, HostRange{c.dpost, (size_t)(width * e)},
+                     HostRange{c.dnext, (size_t)(width * e)}, HostRange{workspace, c.ws.bytes});
+    if (dtype == TPB200_F32) return backward_call<float>(c, st);
+    if (dtype == TPB200_BF16) return backward_call<__nv_bfloat16>(c, st);
+    return backward_call<__half>(c, st);
+}
+
+extern "C" size_t tpb200_rms_norm_backward_workspace_bytes(int64_t outer, int64_t inner, int64_t width) {
+    return tpb200_block_residual_backward_workspace_bytes(outer, inner, width, 0, 1, TPB200_GATE_NONE);
+}
+
+extern "C" int tpb200_rms_norm_backward(const void* grad_y, const int64_t* grad_strides, const void* x, const int64_t* strides, int dtype,
+                                        int64_t outer, int64_t inner, int64_t width, const void* weight, const float* rstd, void* grad_x,
+                                        void* grad_weight, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!weight && outer * inner * width != 0) return fail(TPB200_ERR_INVALID, "rms_norm_backward: NULL pointer argument");
+    return tpb200_block_residual_backward(nullptr, nullptr, grad_y, grad_strides, nullptr, nullptr, x, strides, nullptr, nullptr, TPB200_GATE_NONE,
+                                          nullptr, weight, nullptr, rstd, dtype, outer, inner, width, 1.0, 0.0, 0, 0, grad_x, nullptr, nullptr,
+                                          grad_weight, nullptr, workspace, workspace_bytes, stream);
+}

@@ -134,6 +134,28 @@ int check_register(cudaStream_t st, const HostRange* r, int n);
 #define TPB_CHECK_RANGES(st, ...) do { } while (0)
 #endif
 
+// ---- the training operators (rows [outer, inner, width] with two row strides, three element types)
+inline int64_t dtype_bytes(int dtype) { return dtype == TPB200_F32 ? 4 : (dtype == TPB200_BF16 || dtype == TPB200_F16 ? 2 : 0); }
+// outer x inner rows of `width` consecutive elements, row (a, b) at a * strides[0] + b * strides[1]
+inline HostRange rows_range(const void* p, int64_t outer, int64_t inner, int64_t width, const int64_t* strides, int64_t elem) {
+    const int64_t sizes[3] = {outer, inner, width}, all[3] = {strides ? strides[0] : 0, strides ? strides[1] : 0, 1};
+    if (!p) return HostRange{nullptr, 0};
+    return view_range(p, 3, sizes, all, (size_t)elem);
+}
+// what all of them check first: type, sizes, and a count of elements that 63 bits hold
+inline int check_rows(const char* what, int dtype, int64_t outer, int64_t inner, int64_t width) {
+    if (dtype_bytes(dtype) == 0) return fail(TPB200_ERR_UNSUPPORTED, "%s: only float32, bfloat16 and float16 are supported (dtype code %d)", what, dtype);
+    if (outer < 0 || inner < 0 || width < 0) return fail(TPB200_ERR_INVALID, "%s: negative size", what);
+    if (outer > 0x7fffffffLL || inner > 0x7fffffffLL || outer * inner > 0x7fffffffLL || width > 0x7fffffffLL)
+        return fail(TPB200_ERR_UNSUPPORTED, "%s: at most 2^31 - 1 rows of at most 2^31 - 1 elements", what);
+    return TPB200_OK;
+}
+#define TPB_TRY_ROWS(what, dtype, outer, inner, width)                                       \
+    do {                                                                                     \
+        const int rc__ = ::tpb::check_rows((what), (dtype), (outer), (inner), (width));      \
+        if (rc__ != TPB200_OK) return rc__;                                                  \
+    } while (0)
+
 inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 inline long long round_up(long long a, long long b) { return ceil_div(a, b) * b; }
 inline int pow2_ceil(long long v) {
