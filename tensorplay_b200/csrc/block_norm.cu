@@ -319,6 +319,180 @@ block_backward_kernel(BackwardArgs<T> k) {
     }
 }
 
+// ---------------------------------------------------------------- staged backward ------------
+// The same for 16-byte aligned rows of 513 to 8192 elements, one eight-element vector per thread: each thread
+// copies its own vectors of the next row into shared memory (cp.async, no barrier: nobody else reads them)
+// while it works on this one, so that the row's two reductions over the CTA do not wait for memory.  ARRAYS
+// vectors a row at most: grad_x, grad_y, x_out, h, gate.
+__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)),
+                 "l"(TPB_CKN(src, 16)), "l"(l2_first()) : "memory");
+}
+template <class T>
+struct Staged {
+    static constexpr int kVec = 8 * sizeof(T) / 16;       // 16-byte pieces of a thread's vector
+    uint4* at;          // this thread's first piece of this stage
+    int nthr;
+    __device__ __forceinline__ void fill(int array, const T* p) const {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) copy_async16(at + (array * kVec + j) * nthr, reinterpret_cast<const uint4*>(p) + j);
+    }
+    __device__ __forceinline__ void read(int array, float* f) const {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) Elem<T>::unpack(at[(array * kVec + j) * nthr], f + j * Elem<T>::N);
+    }
+};
+
+constexpr int kStages = 2;
+constexpr int kStageArrays = 5;
+
+template <class T, bool SUM_GATE>
+__global__ void __launch_bounds__(1024, 1)
+block_backward_staged_kernel(BackwardArgs<T> k) {
+    extern __shared__ __align__(16) uint4 stage_mem[];
+    __shared__ float red[2][2][32];
+    const int tid = threadIdx.x, nthr = blockDim.x, worker = blockIdx.x;
+    const float inv_width = 1.0f / (float)k.width;
+    long long lo, hi;
+    if (k.groups_per_worker > 0) {
+        lo = (long long)worker * k.groups_per_worker * k.group_len;
+        hi = lo + k.groups_per_worker * k.group_len;
+        if (hi > k.rows) hi = k.rows;
+    } else {
+        const long long g = worker / k.splits, s = worker - g * k.splits;
+        lo = s * k.split_len;
+        hi = lo + k.split_len;
+        if (hi > k.group_len) hi = k.group_len;
+        lo += g * k.group_len;
+        hi += g * k.group_len;
+    }
+    const bool mine = tid * 8 < k.width;
+    const int e = tid * 8;
+    // the thread's part of both weights lies behind the stages: 16 float32 registers are not to spare
+    const Staged<T> weights{stage_mem + (size_t)(kStages * kStageArrays * Staged<T>::kVec) * nthr + tid, nthr};
+    const auto stage = [&](long long r) {
+        return Staged<T>{stage_mem + (r & 1) * (size_t)(kStageArrays * Staged<T>::kVec) * nthr + tid, nthr};
+    };
+    const auto prefetch = [&](long long r) {
+        if (r < hi && mine) {
+            const long long a = r / k.inner, b = r - a * k.inner;
+            const Staged<T> st = stage(r);
+            if (k.grad_x.p) st.fill(0, k.grad_x.row(a, b) + e);
+            if (k.next) {
+                st.fill(1, k.grad_y.row(a, b) + e);
+                st.fill(2, k.x_out.row(a, b) + e);
+            }
+            if (k.h.p) st.fill(3, k.h.row(a, b) + e);
+            if (k.gate.p) st.fill(4, k.gate.row(a, b) + e);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    float acc_post[8], acc_next[8], acc_gate[SUM_GATE ? 8 : 1];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        acc_post[c] = acc_next[c] = 0.0f;
+        if (SUM_GATE) acc_gate[c] = 0.0f;
+    }
+    if (mine && k.next) weights.fill(0, k.next + e);
+    if (mine && k.post) weights.fill(1, k.post + e);
+    prefetch(lo);
+    for (long long r = lo; r < hi; ++r) {
+        prefetch(r + 1);
+        const float rstd_next = k.next ? *TPB_CK(&k.rstd_next[r]) : 1.0f, rstd_post = k.post ? *TPB_CK(&k.rstd_post[r]) : 1.0f;
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        const Staged<T> st = stage(r);
+        float t[8], u[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) t[c] = 0.0f;
+        float* sums = red[r & 1][0];
+        if (k.next) {
+            float xh[8], s = 0.0f;
+            if (mine) {
+                st.read(2, xh);
+                st.read(1, u);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    xh[c] *= rstd_next;
+                    acc_next[c] = fmaf(u[c], xh[c], acc_next[c]);
+                }
+                float w[8];
+                weights.read(0, w);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    u[c] *= w[c];
+                    s = fmaf(u[c], xh[c], s);
+                }
+            }
+            const float m = row_add<false>(s, sums) * inv_width;
+            if (mine) {
+                if (k.grad_x.p) st.read(0, t);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) t[c] = fmaf(rstd_next, u[c] - xh[c] * m, t[c]);
+            }
+        } else if (mine && k.grad_x.p) {
+            st.read(0, t);
+        }
+        if (mine) store8(k.dx + r * k.width + e, t);
+        if (k.h.p) {
+            float s = 0.0f, hat[8];
+            if (mine) {
+                st.read(3, hat);
+                factors8<true>(k.drop, r, 0, tid, nthr, k.width, u);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    hat[c] *= rstd_post;
+                    u[c] *= k.scale;
+                    t[c] *= u[c];                                  // scale * factor * t
+                }
+                float w[8];
+                if (k.post) weights.read(1, w);
+                if (k.gate.p) {
+                    float g[8];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) u[c] = u[c] == 0.0f ? 0.0f : (k.post ? hat[c] * w[c] : hat[c]) * t[c];
+                    if (SUM_GATE) {
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) acc_gate[c] += u[c];
+                    } else {
+                        store8(k.dgate + r * k.width + e, u);
+                    }
+                    st.read(4, g);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) t[c] *= g[c];
+                }
+                if (k.post) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        acc_post[c] = fmaf(t[c], hat[c], acc_post[c]);
+                        t[c] *= w[c];
+                        s = fmaf(t[c], hat[c], s);
+                    }
+                }
+            }
+            if (k.post) {
+                const float m = row_add<false>(s, sums + 32) * inv_width;
+                if (mine) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) t[c] = rstd_post * (t[c] - hat[c] * m);
+                }
+            }
+            if (mine) store8(k.dh + r * k.width + e, t);
+            if (SUM_GATE && k.groups_per_worker > 0 && (r + 1) % k.group_len == 0) {   // the group is complete
+                if (mine) store8(k.dgate + (r / k.group_len) * k.width + e, acc_gate);
+#pragma unroll
+                for (int c = 0; c < (SUM_GATE ? 8 : 1); ++c) acc_gate[c] = 0.0f;
+            }
+        }
+        // `sums` alternates by the row: whoever writes it again has passed a barrier of the row between, which
+        // everybody reaches after reading it
+    }
+    if (mine) {
+        if (k.post && k.h.p) store8(k.part_post + (long long)worker * k.width + e, acc_post);
+        if (k.next) store8(k.part_next + (long long)worker * k.width + e, acc_next);
+        if (SUM_GATE && k.groups_per_worker == 0) store8(k.part_gate + (long long)worker * k.width + e, acc_gate);
+    }
+}
+
 // Column sums of the workers' partial sums in a fixed order: 32 columns by 8 slots at a time.
 // blockIdx.y: 0 w_post, 1 w_next, 2 + g the gate's group g (slots g * splits ...).
 template <class T>
@@ -358,6 +532,9 @@ inline RowPlan plan_rows(int64_t width, bool vec) {
     p.threads = p.warp ? 256 : (int)std::min<long long>(1024, round_up(ceil_div(width, 8 * p.nv), 32));
     return p;
 }
+
+// Rows of the staged kernel: two stages of five arrays fit the shared memory (float32: up to 5 K elements).
+template <class T> inline size_t stage_bytes(int64_t width) { return (size_t)(kStages * kStageArrays + 2) * round_up(ceil_div(width, 8), 32) * 8 * sizeof(T); }
 
 // How the rows are shared out for the backward pass; depends on sizes only, for the workspace query.
 struct Sharing {
@@ -416,7 +593,18 @@ int backward_run(const BackwardArgs<T>& k, T* dpost, T* dnext, long long gate_gr
                      aligned16(k.post) && aligned16(k.next) && aligned16(k.dx) && aligned16(k.dh) && aligned16(k.dgate);
     RowPlan p = plan_rows(k.width, vec);
     const dim3 grid((unsigned)(p.warp ? ceil_div(k.workers, p.threads / 32) : k.workers));
-    TPB_BLOCK_LAUNCH(block_backward_kernel, T, p, grid, st, k);
+    const size_t smem = stage_bytes<T>(k.width);
+    if (vec && !p.warp && p.nv == 1 && smem <= 220 * 1024) {
+        if (k.gate.p && !k.gate_rows) {
+            TPB_CUDA_OK(cudaFuncSetAttribute(block_backward_staged_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            TPB_LAUNCH("block_backward_staged_kernel", (block_backward_staged_kernel<T, true>), grid, p.threads, smem, st, k);
+        } else {
+            TPB_CUDA_OK(cudaFuncSetAttribute(block_backward_staged_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            TPB_LAUNCH("block_backward_staged_kernel", (block_backward_staged_kernel<T, false>), grid, p.threads, smem, st, k);
+        }
+    } else {
+        TPB_BLOCK_LAUNCH(block_backward_kernel, T, p, grid, st, k);
+    }
     const bool sum_gate = k.gate.p && !k.gate_rows && k.groups_per_worker == 0;
     if (!dpost && !dnext && !sum_gate) return TPB200_OK;
     const dim3 sums((unsigned)ceil_div(k.width, 32), (unsigned)(2 + (sum_gate ? gate_groups : 0)));
@@ -528,7 +716,7 @@ extern "C" int tpb200_rms_norm(const void* x, int dtype, int64_t outer, int64_t 
     if (outer * inner * width == 0) return TPB200_OK;
     if (!x || !strides || !weight || !y || !rstd) return fail(TPB200_ERR_INVALID, "rms_norm: NULL pointer argument");
     cudaStream_t st = (cudaStream_t)stream;
-    const int64_t e = dtype_bytes(dtype), n = outer * inner;
+    [[maybe_unused]] const int64_t e = dtype_bytes(dtype), n = outer * inner;
     TPB_CHECK_RANGES(st, rows_range(x, outer, inner, width, strides, e), HostRange{weight, (size_t)(width * e)}, HostRange{y, (size_t)(n * width * e)},
                      HostRange{rstd, (size_t)n * 4});
     const DropSpec none{0, 0, 0, 1.0f};
@@ -550,7 +738,7 @@ extern "C" int tpb200_block_residual(const void* x, const int64_t* x_strides, co
     if (!x || !h || !x_out || !x_strides || !h_strides || (gate && !gate_strides) || (post_weight && !rstd_post) || (next_weight && (!y || !rstd_next)))
         return fail(TPB200_ERR_INVALID, "block_residual: NULL pointer argument");
     cudaStream_t st = (cudaStream_t)stream;
-    const int64_t e = dtype_bytes(dtype), n = outer * inner;
+    [[maybe_unused]] const int64_t e = dtype_bytes(dtype), n = outer * inner;
     TPB_CHECK_RANGES(st, rows_range(x, outer, inner, width, x_strides, e), rows_range(h, outer, inner, width, h_strides, e),
                      rows_range(gate, outer, inner, width, gate_strides, e), HostRange{post_weight, (size_t)(width * e)},
                      HostRange{next_weight, (size_t)(width * e)}, HostRange{x_out, (size_t)(n * width * e)}, HostRange{y, y ? (size_t)(n * width * e) : 0},

@@ -6,11 +6,13 @@
 //     m = max_j x_j,   s = sum_j 2^(c (x_j - m)),   lse = m + log2(s) / c,   logp = x_y - lse
 //     d logp / d x_j = [j = y] - p_j,   p_j = 2^(c (x_j - m)) / s
 // so every loss that depends on x through logp alone has the gradient coef * ([j = y] - p_j) with one
-// number `coef` per row.  x - m is formed before it is multiplied: a single fused multiply-add c x - c m
-// would save an instruction but loses every digit where the logits themselves are huge, as rows of a
-// type's lowest value are.  c is the float32 nearest to log2(e) and is divided out again in 64 bits.
-//   * s is kept in float32 per thread (a few hundred terms) and joined in float64;
-//   * the per-row scalars (log2 s, logp, differences of log-probabilities) are formed in float64 from an
+// number `coef` per row.  c is the float32 nearest to log2(e) and is divided out again in 64 bits.  m may be any
+// reference near the maximum.  The hot loops take the exponent as one fused multiply-add, c x - M with
+// M = fl(c m): the product is exact there, and M's own rounding, c m - M, is one factor per row (or thread) that
+// is taken out once.  Where |m| >= 2^28 that factor leaves the range of float32 (rows of a type's lowest
+// value are such rows); there x - m is formed first.
+//   * s is kept in float32, a few hundred terms per thread at most, and joined by trees;
+//   * the per-row scalars (log s, logp, differences of log-probabilities) are formed in float64 from an
 //     exponent and a mantissa, the gradient at the token itself is coef * -expm1(logp), which keeps its
 //     digits where p_y is near 1.
 // A token with a negative label or a weight of zero takes no part: its row is not read, its outputs and
@@ -19,9 +21,13 @@
 #include "host_util.h"
 #include "lowp.cuh"
 
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 namespace tpb {
+
+namespace cg = cooperative_groups;
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -29,6 +35,53 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two float32 operations per instruction (sm_100a): differences, products and sums of the sweeps.
+struct __align__(8) Two { float a, b; };
+__device__ __forceinline__ unsigned long long bits_of(float a, float b) {
+    return (unsigned long long)__float_as_uint(a) | ((unsigned long long)__float_as_uint(b) << 32);
+}
+__device__ __forceinline__ Two two_of(unsigned long long v) {
+    return Two{__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long x, unsigned long long y) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long x, unsigned long long y) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+
+__device__ __forceinline__ unsigned long long fma2(unsigned long long x, unsigned long long y, unsigned long long z) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+
+// v[i] := 2^(c v[i] - M), or 2^(c (v[i] - m)), for an even number of values
+template <int N>
+__device__ __forceinline__ void exps_fma(float (&v)[N], float M) {
+    const unsigned long long neg = bits_of(-M, -M), c = bits_of(kLog2e, kLog2e);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const Two t = two_of(fma2(bits_of(v[i], v[i + 1]), c, neg));
+        v[i] = ex2(t.a);
+        v[i + 1] = ex2(t.b);
+    }
+}
+template <int N>
+__device__ __forceinline__ void exps(float (&v)[N], float m) {
+    const unsigned long long neg = bits_of(-m, -m), c = bits_of(kLog2e, kLog2e);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const Two t = two_of(mul2(add2(bits_of(v[i], v[i + 1]), neg), c));
+        v[i] = ex2(t.a);
+        v[i + 1] = ex2(t.b);
+    }
 }
 
 // A float32 (or label) for every token (a, b), at a * s0 + b * s1; strides of 0 broadcast.
@@ -46,63 +99,19 @@ struct Logits {
     int vocab;
 };
 
-// Running (maximum, sum of 2^(c (x - maximum))) of a set of values; the empty set is (-inf, 0).
-struct ExpSum {
-    float m, s;
-    __device__ __forceinline__ void init() { m = -INFINITY; s = 0.0f; }
-    template <int N>
-    __device__ __forceinline__ void add(const float (&v)[N]) {
-        float top = v[0];
-#pragma unroll
-        for (int i = 1; i < N; ++i) top = fmaxf(top, v[i]);     // NaN is never the maximum; it reaches the sum below
-        if (top > m) {
-            s *= ex2((m - top) * kLog2e);
-            m = top;
-        }
-        float t = 0.0f;
-        if (m == -INFINITY) {   // only -inf (and NaN) so far: nothing to add but a NaN
-#pragma unroll
-            for (int i = 0; i < N; ++i) t += v[i];
-            if (t != t) s = NAN;
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) t += ex2((v[i] - m) * kLog2e);
-        s += t;
-    }
-};
-
-struct RowStats { float m; double s; };
-
-// The pairs of all threads of the CTA as one; every thread gets it.
-__device__ __forceinline__ RowStats join_block(const ExpSum& e, float* red_m, double* red_s) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    float m = e.m;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, d));
-    if (lane == 0) red_m[warp] = m;
-    __syncthreads();
-    m = lane < nw ? red_m[lane] : -INFINITY;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, d));
-    // a thread that saw nothing but -inf passes its sum (0 or NaN) as it is
-    double s = warp_add((double)(e.m == -INFINITY ? e.s : e.s * ex2((e.m - m) * kLog2e)));
-    if (lane == 0) red_s[warp] = s;
-    __syncthreads();
-    s = warp_add(lane < nw ? red_s[lane] : 0.0);
-    return RowStats{m, s};
+// log(s) of a row's sum (float32 or joined in float64, rounded to float32 here: 2^-25 of it): the exponent
+// and the logarithm of a mantissa in [1/sqrt 2, sqrt 2), so that the float32 part is below 0.35.  In base
+// 2^(1/c) the logarithm is that of log2(s) / c.  No float64 division on the way: one costs a row some 0.5 us.
+__device__ __forceinline__ double log_sum(float s) {
+    if (!(s >= 1.17549435e-38f && s < INFINITY)) return (double)logf(s);   // 0, NaN, inf
+    int e = (int)(__float_as_uint(s) >> 23) - 127;
+    float f = __uint_as_float((__float_as_uint(s) & 0x007fffffu) | 0x3f800000u);
+    if (f > 1.41421356f) { f *= 0.5f; ++e; }
+    constexpr double kLn2 = 1.0 / (double)kLog2e;       // of the c that the sweeps use
+    return fma((double)e, kLn2, (double)log1pf(f - 1.0f));
 }
 
-// log2 of a positive double: exponent and the float32 logarithm of a mantissa in [1/sqrt 2, sqrt 2)
-__device__ __forceinline__ double log2_split(double s) {
-    if (!(s > 0.0) || s > 1e300) return (double)log2f((float)s);   // 0, NaN, inf
-    int e = (int)((__double_as_longlong(s) >> 52) & 0x7ff) - 1023;
-    double f = __longlong_as_double((__double_as_longlong(s) & 0x000fffffffffffffLL) | 0x3ff0000000000000LL);
-    if (f > 1.4142135623730951) { f *= 0.5; ++e; }
-    return (double)e + (double)(log1pf((float)(f - 1.0)) * kLog2e);
-}
-
-__device__ __forceinline__ double lse_of(const RowStats& r) { return (double)r.m + log2_split(r.s) / (double)kLog2e; }
+__device__ __forceinline__ double lse_of(float m, float s) { return (double)m + log_sum(s); }
 
 // ---------------------------------------------------------------- sweeps over one row --------
 // A row is a head up to the first 16-byte boundary, vectors, and a tail.
@@ -118,46 +127,45 @@ struct Span {
     }
 };
 
-template <class T>
-__device__ __forceinline__ void sweep_stats(const T* p, int len, ExpSum& acc) {
-    constexpr int N = Elem<T>::N;
-    const Span<T> sp(p, len);
-    const int tid = threadIdx.x, nthr = blockDim.x;
-    const T* q = p + sp.head;
-    int i = tid;
-    for (; i + 3 * nthr < sp.nvec; i += 4 * nthr) {
-        uint4 raw[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) raw[u] = ld_once16(q + (size_t)(i + u * nthr) * N);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            float v[N];
-            Elem<T>::unpack(raw[u], v);
-            acc.add(v);
-        }
-    }
-    for (; i < sp.nvec; i += nthr) {
-        float v[N];
-        Elem<T>::unpack(ld_once16(q + (size_t)i * N), v);
-        acc.add(v);
-    }
-    if (tid < sp.head) {
-        float v[1] = {Elem<T>::get(*TPB_CK(&p[tid]))};
-        acc.add(v);
-    }
-    if (tid < sp.tail) {
-        float v[1] = {Elem<T>::get(*TPB_CK(&p[len - 1 - tid]))};
-        acc.add(v);
-    }
-}
+constexpr float kFar = 268435456.0f;     // 2^28
+// c m - M for M = fl(c m): the rounding of M, exactly
+__device__ __forceinline__ float residue(float m, float M) { return fmaf(m, kLog2e, -M); }
 
-// What the gradient of one row needs: g_j = k * 2^(c (x_j - m)), and `at_label` in the token's place.
+// What the gradient of one row needs: g_j = k * 2^(c x_j - M), or k * 2^(c (x_j - m)) for a far row, and
+// `at_label` in the token's place.
 struct RowGrad {
-    float m, k, at_label;
-    int label;
+    float m, M, k, at_label;
+    int label, far;
+    // from the reference, the sum of 2^(c (x - m)) (its reciprocal), the coefficient and logp
+    __device__ __forceinline__ void set(float reference, float inv_s, float coef, float logp, int at) {
+        m = reference;
+        far = !(fabsf(m) < kFar);
+        M = far ? 0.0f : m * kLog2e;
+        k = -coef * inv_s;
+        if (!far) k *= ex2(-residue(m, M));
+        at_label = coef * -expm1f(logp);
+        label = at;
+    }
+    __device__ __forceinline__ float value(float x) const { return k * ex2(far ? (x - m) * kLog2e : fmaf(x, kLog2e, -M)); }
 };
-__device__ __forceinline__ float grad_at(float x, int j, const RowGrad& g) {
-    return j == g.label ? g.at_label : g.k * ex2((x - g.m) * kLog2e);
+__device__ __forceinline__ float grad_at(float x, int j, const RowGrad& g) { return j == g.label ? g.at_label : g.value(x); }
+
+// k * 2^(c x - M) of a vector
+template <class T>
+__device__ __forceinline__ uint4 grad_vector(const uint4& raw, const RowGrad& g, bool far) {
+    constexpr int N = Elem<T>::N;
+    float v[N];
+    Elem<T>::unpack(raw, v);
+    if (far) exps(v, g.m);
+    else exps_fma(v, g.M);
+    const unsigned long long k = bits_of(g.k, g.k);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const Two t = two_of(mul2(bits_of(v[i], v[i + 1]), k));
+        v[i] = t.a;
+        v[i + 1] = t.b;
+    }
+    return Elem<T>::pack(v);
 }
 
 template <class T>
@@ -203,72 +211,6 @@ struct RowLimits {
     }
 };
 
-// logp and lse of every row; `keep` (a workspace, may be NULL) gets (m, 1 / s) for the gradient.
-template <class T>
-__global__ void __launch_bounds__(512)
-score_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, float* __restrict__ logp, float* __restrict__ lse,
-             float2* __restrict__ keep) {
-    __shared__ float red_m[32];
-    __shared__ double red_s[32];
-    const long long r = blockIdx.x, a = r / in.inner, b = r - a * in.inner;
-    const long long y = labels.at(a, b);
-    if (y < 0 || !limits.inside(r)) {
-        if (threadIdx.x == 0) {
-            *TPB_CK(&logp[r]) = 0.0f;
-            if (lse) *TPB_CK(&lse[r]) = 0.0f;
-            if (keep) *TPB_CK(&keep[r]) = make_float2(0.0f, 0.0f);
-        }
-        return;
-    }
-    const T* p = in.x + a * in.s0 + b * in.s1;
-    ExpSum acc;
-    acc.init();
-    sweep_stats(p, in.vocab, acc);
-    const RowStats st = join_block(acc, red_m, red_s);
-    if (threadIdx.x == 0) {
-        const double n = lse_of(st);
-        *TPB_CK(&logp[r]) = y < in.vocab ? (float)((double)Elem<T>::get(*TPB_CK(&p[y])) - n) : NAN;
-        if (lse) *TPB_CK(&lse[r]) = (float)n;
-        if (keep) *TPB_CK(&keep[r]) = make_float2(st.m, (float)(1.0 / st.s));
-    }
-}
-
-// ---------------------------------------------------------------- gradient from saved statistics
-// coef of every row from the caller's grad_logp (with lse), or from a workspace (with keep).
-template <class T>
-__global__ void __launch_bounds__(512)
-score_grad_kernel(Logits<T> in, PerToken<long long> labels, PerToken<float> grad_logp, const float* __restrict__ lse,
-                  const float2* __restrict__ keep, const float* __restrict__ coefs, const float* __restrict__ logp,
-                  T* __restrict__ out) {
-    const long long r = blockIdx.x, a = r / in.inner, b = r - a * in.inner;
-    T* o = out + r * (long long)in.vocab;
-    const long long y = labels.at(a, b);
-    const float coef = y < 0 ? 0.0f : (coefs ? *TPB_CK(&coefs[r]) : grad_logp.at(a, b));
-    if (coef == 0.0f) {
-        sweep_zero(o, in.vocab);
-        return;
-    }
-    const T* p = in.x + a * in.s0 + b * in.s1;
-    RowGrad g;
-    float lp;
-    if (keep) {
-        const float2 k = *TPB_CK(&keep[r]);
-        g.m = k.x;
-        g.k = -coef * k.y;
-        lp = *TPB_CK(&logp[r]);
-    } else {
-        // p = 2^(c (x - lse))
-        const double L = (double)*TPB_CK(&lse[r]);
-        g.m = (float)L;
-        g.k = -coef;
-        lp = y < in.vocab ? (float)((double)Elem<T>::get(*TPB_CK(&p[y])) - L) : NAN;
-    }
-    if (y >= in.vocab) g.k = NAN;
-    g.label = y < in.vocab ? (int)y : -1;
-    g.at_label = coef * -expm1f(lp);
-    sweep_grad(p, o, in.vocab, g);
-}
-
 // ---------------------------------------------------------------- clipped policy loss ---------
 struct PolicyTerms {
     PerToken<float> old_logp, advantage, weight, ref;   // ref.p may be NULL
@@ -298,68 +240,407 @@ __device__ __forceinline__ float kl_term(float d) {
     return expm1f(d) - d;
 }
 
+// A token's inputs, fetched before the row is swept.
+struct PolicyToken { float old_logp, advantage, weight, ref; };
+__device__ __forceinline__ PolicyToken policy_token(const PolicyTerms& t, long long a, long long b, float w) {
+    return PolicyToken{t.old_logp.at(a, b), t.advantage.at(a, b), w, t.ref.p ? t.ref.at(a, b) : 0.0f};
+}
+
 // The row's outputs and its coefficient d loss / d logp:
 //   l = -min(r A, clip(r, 1 - low, 1 + high) A) + kl_coef (e^d - d - 1),  r = e^(logp - old), d = ref - logp
 //   dl / d logp = -r A (where the unclipped branch is the smaller one) + kl_coef (1 - e^d)
-__device__ __forceinline__ float policy_row(const PolicyTerms& t, const PolicyOut& out, long long r, long long a, long long b,
-                                            double logp, float w) {
-    const float adv = t.advantage.at(a, b);
-    const float ratio = expf((float)(logp - (double)t.old_logp.at(a, b)));
-    const float free_gain = ratio * adv;
-    const float held = fminf(fmaxf(ratio, 1.0f - t.low), 1.0f + t.high) * adv;
+struct PolicyRow { float ratio, kl, coef; double part; };
+__device__ __forceinline__ PolicyRow policy_row(const PolicyTerms& t, const PolicyToken& k, double logp) {
+    PolicyRow o;
+    o.ratio = expf((float)(logp - (double)k.old_logp));
+    const float free_gain = o.ratio * k.advantage;
+    const float held = fminf(fmaxf(o.ratio, 1.0f - t.low), 1.0f + t.high) * k.advantage;
     // not (held < free): NaN keeps the unclipped branch, and with it the NaN
     const bool clipped = held < free_gain;
-    float loss = -(clipped ? held : free_gain), slope = clipped ? 0.0f : -free_gain, kl = 0.0f;
+    float loss = -(clipped ? held : free_gain), slope = clipped ? 0.0f : -free_gain;
+    o.kl = 0.0f;
     if (t.ref.p) {
-        const float d = (float)((double)t.ref.at(a, b) - logp);
-        kl = kl_term(d);
-        loss = fmaf(t.kl_coef, kl, loss);
+        const float d = (float)((double)k.ref - logp);
+        o.kl = kl_term(d);
+        loss = fmaf(t.kl_coef, o.kl, loss);
         slope = fmaf(t.kl_coef, -expm1f(d), slope);
     }
+    o.part = (double)k.weight * (double)loss;
+    o.coef = k.weight * slope * t.grad_scale;
+    return o;
+}
+__device__ __forceinline__ void store_policy(const PolicyOut& out, long long r, double logp, const PolicyRow& o) {
     *TPB_CK(&out.logp[r]) = (float)logp;
-    *TPB_CK(&out.ratio[r]) = ratio;
-    *TPB_CK(&out.kl[r]) = kl;
-    *TPB_CK(&out.part[r]) = (double)w * (double)loss;
-    return w * slope * t.grad_scale;
+    *TPB_CK(&out.ratio[r]) = o.ratio;
+    *TPB_CK(&out.kl[r]) = o.kl;
+    *TPB_CK(&out.part[r]) = o.part;
 }
 
+// ---------------------------------------------------------------- sweeps of a part of a row ---
+// The part of a row that CTA `rank` of `C` takes: `n` vectors from vector `first` behind the head.
 template <class T>
-__global__ void __launch_bounds__(512)
-policy_kernel(Logits<T> in, PerToken<long long> labels, PolicyTerms terms, PolicyOut out, T* __restrict__ grad) {
-    __shared__ float red_m[32];
-    __shared__ double red_s[32];
-    __shared__ RowGrad sh;
-    const long long r = blockIdx.x, a = r / in.inner, b = r - a * in.inner;
-    const long long y = labels.at(a, b);
-    const float w = terms.weight.at(a, b);
-    T* o = grad ? grad + r * (long long)in.vocab : nullptr;
-    if (y < 0 || w == 0.0f) {
-        if (threadIdx.x == 0) {
-            *TPB_CK(&out.logp[r]) = 0.0f;
-            *TPB_CK(&out.ratio[r]) = 0.0f;
-            *TPB_CK(&out.kl[r]) = 0.0f;
-            *TPB_CK(&out.part[r]) = 0.0;
+struct Part {
+    int head, tail, nvec, first, n;
+    __device__ __forceinline__ Part(const T* p, int len, int rank, int C) {
+        const Span<T> sp(p, len);
+        head = sp.head;
+        tail = sp.tail;
+        nvec = sp.nvec;
+        const int each = (nvec + C - 1) / C;
+        first = min(rank * each, nvec);
+        n = min(each, nvec - first);
+    }
+    // the element outside of the vectors that this thread takes (the CTA has at least 32 threads), or -1
+    __device__ __forceinline__ int edge(int tid, int len, int rank, int C) const {
+        if (rank == 0 && tid < head) return tid;
+        if (rank == C - 1 && tid >= 16 && tid - 16 < tail) return len - 1 - (tid - 16);
+        return -1;
+    }
+};
+
+template <class T>
+__device__ __forceinline__ void zero_part(T* o, const Part<T>& z, int len, int rank, int C) {
+    constexpr int N = Elem<T>::N;
+    const int tid = threadIdx.x;
+    for (int i = tid; i < z.n; i += blockDim.x) st_out16(o + z.head + (size_t)(z.first + i) * N, make_uint4(0, 0, 0, 0));
+    const int e = z.edge(tid, len, rank, C);
+    if (e >= 0) *TPB_CK(&o[e]) = Elem<T>::put(0.0f);
+}
+
+// Maximum of a vector's elements and `m`, on packed pairs for the 16-bit types; NaN is never the maximum.
+template <class T> struct VecMax;
+template <> struct VecMax<float> {
+    float m = -INFINITY;
+    __device__ __forceinline__ void add(const uint4& v) {
+        m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w))));
+    }
+    __device__ __forceinline__ float get() const { return m; }
+};
+template <> struct VecMax<__nv_bfloat16> {
+    __nv_bfloat162 m = __nv_bfloat162{__ushort_as_bfloat16(0xff80), __ushort_as_bfloat16(0xff80)};
+    static __device__ __forceinline__ __nv_bfloat162 of(uint32_t w) { __nv_bfloat162 r; memcpy(&r, &w, 4); return r; }
+    __device__ __forceinline__ void add(const uint4& v) { m = __hmax2(m, __hmax2(__hmax2(of(v.x), of(v.y)), __hmax2(of(v.z), of(v.w)))); }
+    __device__ __forceinline__ float get() const { return fmaxf(__low2float(m), __high2float(m)); }
+};
+template <> struct VecMax<__half> {
+    __half2 m = __half2{__ushort_as_half(0xfc00), __ushort_as_half(0xfc00)};
+    static __device__ __forceinline__ __half2 of(uint32_t w) { __half2 r; memcpy(&r, &w, 4); return r; }
+    __device__ __forceinline__ void add(const uint4& v) { m = __hmax2(m, __hmax2(__hmax2(of(v.x), of(v.y)), __hmax2(of(v.z), of(v.w)))); }
+    __device__ __forceinline__ float get() const { return fmaxf(__low2float(m), __high2float(m)); }
+};
+
+// Running sum of 2^(c x - M) of one thread over a row, two vectors at a time, against a reference that is fixed
+// after the first of them: no maximum and no rescaling per element.  A step whose sum is not below 2^60 --
+// values far above the reference, infinities, NaN, far rows (their M is NaN) -- is done again the careful
+// way, which raises the reference.  (A running maximum took 25 instructions per element in all, this 14.)
+template <class T>
+struct FixedSum {
+    static constexpr int N = Elem<T>::N;
+    float ref, M, s;      // ref = -inf: nothing but -inf and NaN so far; M = NaN then, and for a far reference
+    __device__ __forceinline__ void init() { ref = -INFINITY; M = NAN; s = 0.0f; }
+    // s relative to 2^(c ref) rather than 2^M, and back
+    __device__ __forceinline__ float out(float v) const { return M != M ? v : v * ex2(-residue(ref, M)); }
+    __device__ __forceinline__ float in(float v) const { return M != M ? v : v * ex2(residue(ref, M)); }
+    __device__ __forceinline__ void refer(float high) {
+        ref = high;
+        M = fabsf(ref) < kFar ? ref * kLog2e : NAN;
+    }
+    static __device__ __noinline__ FixedSum careful(FixedSum f, uint4 raw) {
+        VecMax<T> top;
+        top.add(raw);
+        const float high = top.get();
+        if (high > f.ref) {
+            const float r = f.out(f.s) * ex2((f.ref - high) * kLog2e);     // 0 * 0 at the start
+            f.refer(high);
+            f.s = f.in(r);
         }
-        if (o) sweep_zero(o, in.vocab);
-        return;
+        float t = 0.0f, v[N];
+        Elem<T>::unpack(raw, v);
+#pragma unroll
+        for (int i = 0; i < N; ++i) t += f.ref == -INFINITY ? (v[i] != v[i] ? NAN : 0.0f) : ex2((v[i] - f.ref) * kLog2e);
+        f.s += f.in(t);
+        return f;
     }
-    const T* p = in.x + a * in.s0 + b * in.s1;
-    ExpSum acc;
-    acc.init();
-    sweep_stats(p, in.vocab, acc);
-    const RowStats st = join_block(acc, red_m, red_s);
-    if (threadIdx.x == 0) {
-        const double logp = y < in.vocab ? (double)Elem<T>::get(*TPB_CK(&p[y])) - lse_of(st) : (double)NAN;
-        const float coef = policy_row(terms, out, r, a, b, logp, w);
-        sh.m = st.m;
-        sh.k = (float)(-(double)coef / st.s);
-        sh.label = y < in.vocab ? (int)y : -1;
-        sh.at_label = coef * -expm1f((float)logp);
+    template <int VECS>
+    __device__ __forceinline__ void add(const uint4 (&raw)[VECS], bool first = false) {
+        if (first) {
+            VecMax<T> top;
+#pragma unroll
+            for (int u = 0; u < VECS; ++u) top.add(raw[u]);
+            refer(top.get());
+        }
+        unsigned long long t2 = 0;
+#pragma unroll
+        for (int u = 0; u < VECS; ++u) {
+            float v[N];
+            Elem<T>::unpack(raw[u], v);
+            exps_fma(v, M);
+#pragma unroll
+            for (int i = 0; i < N; i += 2) t2 = add2(t2, bits_of(v[i], v[i + 1]));
+        }
+        const Two h = two_of(t2);
+        const float t = h.a + h.b;
+        if (t < 1.1529215e18f) {
+            s += t;
+        } else {
+#pragma unroll
+            for (int u = 0; u < VECS; ++u) *this = careful(*this, raw[u]);
+        }
     }
-    if (!o) return;
+};
+
+// Where the output's 16-byte boundaries lie `k` elements (1 .. N - 1) behind those of the input: the vector that
+// ends at the boundary inside a lane's own vector, from the last N - k elements of the vector before it and
+// the first k of its own.
+template <class T>
+__device__ __forceinline__ uint4 straddle(const uint4& before, const uint4& own, int k) {
+    const int bits = k * (int)sizeof(T) * 8;      // the same for the whole row
+    uint32_t w[8] = {before.x, before.y, before.z, before.w, own.x, own.y, own.z, own.w};
+    if (bits & 64) {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (bits & 32) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    const int sh = bits & 31;
+    return make_uint4(__funnelshift_r(w[0], w[1], sh), __funnelshift_r(w[1], w[2], sh), __funnelshift_r(w[2], w[3], sh),
+                      __funnelshift_r(w[3], w[4], sh));
+}
+
+// The gradient of one CTA's part of a row.  FAR and the alignment of the output are the same for the whole row.
+template <class T>
+__device__ __forceinline__ void grad_part(const T* p, T* o, const Part<T>& part, const RowGrad& g, int edge, float edge_x) {
+    constexpr int N = Elem<T>::N;
+    const int tid = threadIdx.x, lane = tid & 31, nthr = blockDim.x;
+    const T* q = p + part.head + (size_t)part.first * N;
+    T* t = o + part.head + (size_t)part.first * N;
+    const int shift = (int)(((16 - ((uintptr_t)t & 15)) & 15) / sizeof(T));    // elements up to a 16-byte boundary
+    int lo = tid, hi = part.n, step = nthr;         // this thread's vectors: lo, lo + step, ... below hi
+    if (shift == 0 && !g.far) {
+        for (int i = lo; i < hi; i += step) st_out16(t + (size_t)i * N, grad_vector<T>(ld_once16(q + (size_t)i * N), g, false));
+    } else if (shift == 0) {
+        for (int i = lo; i < hi; i += step) st_out16(t + (size_t)i * N, grad_vector<T>(ld_once16(q + (size_t)i * N), g, true));
+    } else {
+        // a run of consecutive vectors for every warp; what is left over at its two ends goes out one by one
+        const int run = (part.n + nthr - 1) / nthr * 32;
+        lo = min((tid >> 5) * run, part.n) + lane;
+        hi = min(lo - lane + run, part.n);
+        step = 32;
+        uint4 last = make_uint4(0, 0, 0, 0);
+        for (int i = lo; i - lane < hi; i += 32) {
+            const uint4 v = grad_vector<T>(i < hi ? ld_once16(q + (size_t)i * N) : make_uint4(0, 0, 0, 0), g, g.far);
+            const uint4 give = lane == 31 ? last : v;       // lane 0 follows lane 31 of the step before
+            uint4 before;
+            before.x = __shfl_sync(kFull, give.x, (lane + 31) & 31);
+            before.y = __shfl_sync(kFull, give.y, (lane + 31) & 31);
+            before.z = __shfl_sync(kFull, give.z, (lane + 31) & 31);
+            before.w = __shfl_sync(kFull, give.w, (lane + 31) & 31);
+            T* at = t + (size_t)i * N;
+            const bool first = i == lo && lane == 0, end = i == hi - 1;
+            if (i < hi && !first) st_out16(at + shift - N, straddle<T>(before, v, shift));
+            if ((first && i < hi) || end) {
+                union { uint4 u; T e[N]; } x;
+                x.u = v;
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (e < shift ? first : end) *TPB_CK(&at[e]) = x.e[e];
+            }
+            last = v;
+        }
+    }
+    if (edge >= 0) *TPB_CK(&o[edge]) = Elem<T>::put(grad_at(edge_x, edge, g));
+    // the token's own entry, over what this warp has just stored there
+    __syncwarp();
+    if (g.label >= part.head && g.label < part.head + part.nvec * N) {
+        const int i = (g.label - part.head) / N - part.first;
+        if (i >= lo && i < hi && (i - lo) % step == 0) *TPB_CK(&o[g.label]) = Elem<T>::put(g.at_label);
+    }
+}
+
+struct ScoreOut {
+    float *logp, *lse;   // all but logp may be NULL
+    float2* keep;        // (reference, 1 / s)
+    double* exact;       // logp before it is rounded
+};
+
+// (sum, reference) pairs of the lanes as one
+__device__ __forceinline__ void join_warp(float& s, float& m) {
+    const float own = m;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, d));
+    s = warp_add(own == -INFINITY ? s : s * ex2((own - m) * kLog2e));     // -inf: 0, or NaN for a NaN
+}
+
+constexpr int kRowThreads = 512;
+#ifdef TPB200_CHECKED
+constexpr int kRowCtas = 3;      // on an SM; the checker's own function needs 38 registers
+#else
+constexpr int kRowCtas = 4;
+#endif
+constexpr int kRowCluster = 8;
+
+// Log-probabilities, and with POLICY the whole policy loss: a cluster of C CTAs per row, each with 1/C of the
+// row's 16-byte vectors.  The first sweep sums, the CTAs' (sum, reference) pairs cross the cluster through
+// distributed shared memory, and the second sweep writes the gradient; it reads the row again, from L2,
+// because C is chosen so that the rows in flight take half of it (row_shape), and because loads and stores say
+// what may be evicted.  Bytes from and to memory are then near one read and one write.  What bounds it: two
+// ex2 per element, 16 a cycle on an SM (249 of 360 us on [4096,151936] bf16 with 90 % of the rows counted), nine
+// instructions per element, and the second read through L2; 2048 threads on an SM hide their latencies.
+// Measured, of one read and one write: [4096,50016] bf16 4.97 TB/s (C = 1), [1024,151936] bf16 4.46 (C = 3),
+// f32 4.83 (C = 6); with two CTAs of 512 on an SM instead of four 4.0, 4.0 and 4.3; in separate kernels for
+// sum and gradient 3.8 and 3.8.  Keeping the row in shared memory instead (a ring of bulk copies, persistent CTAs)
+// left 16 to 26 warps on an SM to hide the latencies and was slower: 4.6, 4.0 and 3.2.
+template <class T, bool POLICY>
+__global__ void __launch_bounds__(kRowThreads, kRowCtas)
+row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTerms terms, PolicyOut out, ScoreOut score, T* __restrict__ grad, int C,
+           float* __restrict__ loss) {
+    constexpr int N = Elem<T>::N;
+    __shared__ float red_s[kRowThreads / 32], red_m[kRowThreads / 32];
+    __shared__ float2 pair[kRowCluster];     // (sum, reference) of every CTA of the cluster
+    __shared__ RowGrad sh;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nthr = blockDim.x;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = C > 1 ? (int)cluster.block_rank() : 0;
+    const unsigned r = blockIdx.x / (unsigned)C, a = r / (unsigned)in.inner, b = r - a * (unsigned)in.inner;
+    long long label = labels.at(a, b);
+    float weight = 0.0f;
+    if (POLICY) {
+        weight = terms.weight.at(a, b);
+        if (weight == 0.0f) label = -1;
+    } else if (!limits.inside(r)) {
+        label = -1;
+    }
+    T* o = POLICY && grad ? grad + (long long)r * in.vocab : nullptr;
+    if (label < 0) {
+        if (tid == 0 && rank == 0) {
+            if (POLICY) {
+                store_policy(out, r, 0.0, PolicyRow{0.0f, 0.0f, 0.0f, 0.0});
+                if (loss) *TPB_CK(loss) = 0.0f;
+            } else {
+                *TPB_CK(&score.logp[r]) = 0.0f;
+                if (score.lse) *TPB_CK(&score.lse[r]) = 0.0f;
+                if (score.keep) *TPB_CK(&score.keep[r]) = make_float2(0.0f, 0.0f);
+                if (score.exact) *TPB_CK(&score.exact[r]) = 0.0;
+            }
+        }
+        if (POLICY && o) zero_part(o, Part<T>(o, in.vocab, rank, C), in.vocab, rank, C);
+        return;                             // all CTAs of the cluster alike
+    }
+    const T* p = in.x + (long long)a * in.s0 + (long long)b * in.s1;
+    const Part<T> part(p, in.vocab, rank, C);
+    PolicyToken token{};
+    float at_label = 0.0f;
+    if (tid == 0) {
+        if (POLICY) token = policy_token(terms, a, b, weight);
+        at_label = label < in.vocab ? Elem<T>::get(*TPB_CK(&p[label])) : 0.0f;
+    }
+    const int edge = part.edge(tid, in.vocab, rank, C);
+    const float edge_x = edge >= 0 ? Elem<T>::get(*TPB_CK(&p[edge])) : -INFINITY;
+
+    // ---- the sum
+    const T* q = p + part.head + (size_t)part.first * N;
+    FixedSum<T> sum;
+    sum.init();
+    {
+        // a row that is swept twice stays in L2 until then
+        const unsigned long long policy = POLICY && o ? l2_last() : l2_first();
+        int i = tid;
+        for (; i + nthr < part.n; i += 2 * nthr) {
+            const uint4 raw[2] = {ld_policy16(q + (size_t)i * N, policy), ld_policy16(q + (size_t)(i + nthr) * N, policy)};
+            sum.add(raw, i == tid);
+        }
+        if (i < part.n) {
+            const uint4 raw[1] = {ld_policy16(q + (size_t)i * N, policy)};
+            sum.add(raw, i == tid);
+        }
+        if (edge >= 0) {                    // as a vector with one element
+            float v[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = e == 0 ? edge_x : -INFINITY;
+            const uint4 raw[1] = {Elem<T>::pack(v)};
+            sum.add(raw);
+        }
+    }
+    float m = sum.ref, s = sum.out(sum.s);
+    join_warp(s, m);
+    if (nthr > 32) {
+        if (lane == 0) {
+            red_s[warp] = s;
+            red_m[warp] = m;
+        }
+        __syncthreads();
+        const int nw = nthr >> 5;
+        s = lane < nw ? red_s[lane] : 0.0f;
+        m = lane < nw ? red_m[lane] : -INFINITY;
+        join_warp(s, m);
+    }
+    if (C > 1) {
+        if (tid < C) *cluster.map_shared_rank(&pair[rank], (unsigned)tid) = make_float2(s, m);
+        cluster.sync();
+        const float2 v = lane < C ? pair[lane & (kRowCluster - 1)] : make_float2(0.0f, -INFINITY);
+        s = v.x;
+        m = v.y;
+        join_warp(s, m);                    // the same order in every CTA
+    }
+    if (tid == 0) {
+        const double norm = lse_of(m, s);
+        const double logp = label < in.vocab ? (double)at_label - norm : (double)NAN;
+        if (POLICY) {
+            const PolicyRow row = policy_row(terms, token, logp);
+            sh.set(m, 1.0f / s, row.coef, (float)logp, label < in.vocab ? (int)label : -1);
+            if (rank == 0) {
+                store_policy(out, r, logp, row);
+                if (loss) *TPB_CK(loss) = (float)row.part;
+            }
+        } else if (rank == 0) {
+            *TPB_CK(&score.logp[r]) = (float)logp;
+            if (score.lse) *TPB_CK(&score.lse[r]) = (float)norm;
+            if (score.keep) *TPB_CK(&score.keep[r]) = make_float2(m, 1.0f / s);
+            if (score.exact) *TPB_CK(&score.exact[r]) = logp;
+        }
+    }
+    if (!POLICY || !o) return;
     __syncthreads();
     const RowGrad g = sh;
-    sweep_grad(p, o, in.vocab, g);
+    grad_part(p, o, part, g, edge, edge_x);
+}
+
+// ---------------------------------------------------------------- gradient from saved statistics
+// coef of every row from the caller's grad_logp (with lse), or from a workspace (with keep).
+template <class T>
+__global__ void __launch_bounds__(kRowThreads, kRowCtas)
+score_grad_kernel(Logits<T> in, PerToken<long long> labels, PerToken<float> grad_logp, const float* __restrict__ lse,
+                  const float2* __restrict__ keep, const float* __restrict__ coefs, const float* __restrict__ logp, T* __restrict__ out, unsigned rows,
+                  int C) {
+    // with saved statistics the rows go backwards: the last ones that the sums read are still in L2
+    unsigned r = blockIdx.x / (unsigned)C;
+    const int rank = (int)(blockIdx.x - r * (unsigned)C);
+    if (keep) r = rows - 1 - r;
+    const unsigned a = r / (unsigned)in.inner, b = r - a * (unsigned)in.inner;
+    T* o = out + (long long)r * in.vocab;
+    const long long y = labels.at(a, b);
+    const float coef = y < 0 ? 0.0f : (coefs ? *TPB_CK(&coefs[r]) : grad_logp.at(a, b));
+    if (coef == 0.0f) {
+        zero_part(o, Part<T>(o, in.vocab, rank, C), in.vocab, rank, C);
+        return;
+    }
+    const T* p = in.x + (long long)a * in.s0 + (long long)b * in.s1;
+    const Part<T> part(p, in.vocab, rank, C);
+    const int edge = part.edge(threadIdx.x, in.vocab, rank, C);
+    const float edge_x = edge >= 0 ? Elem<T>::get(*TPB_CK(&p[edge])) : -INFINITY;
+    RowGrad g;
+    const int at = y < in.vocab ? (int)y : -1;
+    if (keep) {
+        const float2 k = *TPB_CK(&keep[r]);
+        g.set(k.x, k.y, coef, *TPB_CK(&logp[r]), at);
+    } else {
+        const float n = *TPB_CK(&lse[r]);      // p = 2^(c (x - lse))
+        g.set(n, 1.0f, coef, y < in.vocab ? (float)((double)Elem<T>::get(*TPB_CK(&p[y])) - (double)n) : NAN, at);
+    }
+    if (y >= in.vocab) g.k = NAN;
+    grad_part(p, o, part, g, edge, edge_x);
 }
 
 // ---------------------------------------------------------------- sums and pairs --------------
@@ -382,7 +663,7 @@ loss_sum_kernel(const double* __restrict__ part, long long n, double factor, flo
 //   margin = beta (s_chosen - s_rejected);  loss = -(1 - e) log sig(margin) - e log sig(-margin)
 //   d loss / d margin = e sig(margin) - (1 - e) sig(-margin)
 __global__ void __launch_bounds__(256)
-pair_kernel(PerToken<long long> labels, PerToken<float> ref, const float* __restrict__ logp, const long long* __restrict__ offsets,
+pair_kernel(PerToken<long long> labels, PerToken<float> ref, const double* __restrict__ logp, const long long* __restrict__ offsets,
             long long rows, long long inner, long long pairs, double beta, double smoothing, double grad_scale,
             float* __restrict__ rewards, double* __restrict__ part, float* __restrict__ coefs) {
     __shared__ double red[8];
@@ -405,7 +686,7 @@ pair_kernel(PerToken<long long> labels, PerToken<float> ref, const float* __rest
         double s = 0.0;
         for (long long r = lo[j] + threadIdx.x; r < hi[j]; r += blockDim.x) {
             const long long a = r / inner, b = r - a * inner;
-            if (labels.at(a, b) >= 0) s += (double)*TPB_CK(&logp[r]) - (double)ref.at(a, b);
+            if (labels.at(a, b) >= 0) s += *TPB_CK(&logp[r]) - (double)ref.at(a, b);
         }
         s = warp_add(s);
         if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
@@ -456,6 +737,45 @@ inline PerToken<float> per_token(const float* p, const int64_t* strides) {
         else { using T = __half; call; }                      \
     } while (0)
 
+// Threads of a CTA and CTAs per row.  Short rows get as many threads as they have pairs of vectors.  More than one
+// CTA per row: with a second sweep, so that the rows in flight (four CTAs on every SM) take at most 60 MB, half
+// of L2; and while the rows alone do not fill the GPU and a CTA still has two vectors per thread.  [1024,151936] bf16,
+// C = 1, 2, 3, 4, 6: 4.10, 4.38, 4.46, 4.33, 3.94 TB/s; f32: 4.12, 4.20, 4.44, 4.44, 4.83.
+struct RowShape { int threads, C; };
+inline RowShape row_shape(int64_t rows, int64_t vocab, int64_t elem, bool twice) {
+    const int64_t vectors = vocab * elem / 16, room = 4LL * sm_count();
+    RowShape s{(int)std::max<int64_t>(32, std::min<int64_t>(kRowThreads, round_up(ceil_div(vectors, 2), 32))), 1};
+    if (s.threads < kRowThreads) return s;
+    int64_t C = 1;
+    if (twice) C = std::min<int64_t>(kRowCluster, ceil_div(std::min(rows, room) * vocab * elem, 60LL << 20));
+    while (C < kRowCluster && rows * C < room && vectors >= (C + 1) * 2 * kRowThreads) ++C;
+    if (rows * C > 0x7fffffffLL) C = 1;
+    s.C = (int)C;
+    return s;
+}
+
+template <class T, bool POLICY>
+int row_run(const Logits<T>& in, const PerToken<long long>& lab, const RowLimits& limits, const PolicyTerms& terms, const PolicyOut& out,
+            const ScoreOut& score, T* grad, int64_t rows, float* loss, cudaStream_t st) {
+    const RowShape s = row_shape(rows, in.vocab, sizeof(T), grad != nullptr);
+    const cudaError_t e = launch_ex(row_kernel<T, POLICY>, dim3((unsigned)(rows * s.C)), s.threads, 0, st, s.C, false, in, lab, limits, terms, out, score, grad,
+                                    s.C, rows == 1 ? loss : nullptr);
+    return e == cudaSuccess ? TPB200_OK : cuda_fail(e, "row_kernel");
+}
+template <class T>
+int score_run(const Logits<T>& in, const PerToken<long long>& lab, const RowLimits& limits, float* logp, float* lse, float2* keep,
+              double* exact, int64_t rows, cudaStream_t st) {
+    return row_run<T, false>(in, lab, limits, PolicyTerms{}, PolicyOut{}, ScoreOut{logp, lse, keep, exact}, (T*)nullptr, rows, nullptr, st);
+}
+template <class T>
+int score_grad_run(const Logits<T>& in, const PerToken<long long>& lab, const PerToken<float>& grad_logp, const float* lse, const float2* keep,
+                   const float* coefs, const float* logp, T* out, int64_t rows, cudaStream_t st) {
+    const RowShape s = row_shape(rows, in.vocab, sizeof(T), false);
+    TPB_LAUNCH("score_grad_kernel", score_grad_kernel<T>, dim3((unsigned)(rows * s.C)), s.threads, 0, st, in, lab, grad_logp, lse, keep, coefs, logp, out,
+               (unsigned)rows, s.C);
+    return TPB200_OK;
+}
+
 int check_logits(const char* what, int dtype, int64_t outer, int64_t inner, int64_t vocab, const void* logits, const int64_t* strides,
                  const int64_t* labels, const int64_t* label_strides) {
     TPB_TRY_ROWS(what, dtype, outer, inner, vocab);
@@ -483,8 +803,7 @@ extern "C" int tpb200_token_logprobs(const void* logits, int dtype, int64_t oute
     TPB_CHECK_RANGES(st, rows_range(logits, outer, inner, vocab, strides, dtype_bytes(dtype)), rows_range(labels, outer, inner, 1, label_strides, 8),
                      HostRange{logp, (size_t)rows * 4}, HostRange{lse, (size_t)rows * 4});
     const PerToken<long long> lab{(const long long*)labels, label_strides[0], label_strides[1]};
-    TPB_BY_TYPE(dtype, TPB_LAUNCH("score_kernel", score_kernel<T>, dim3((unsigned)rows), 512, 0, st,
-                                  logits_of<T>(logits, inner, vocab, strides), lab, RowLimits{nullptr, 0}, logp, lse, nullptr));
+    TPB_BY_TYPE(dtype, return score_run<T>(logits_of<T>(logits, inner, vocab, strides), lab, RowLimits{nullptr, 0}, logp, lse, nullptr, nullptr, rows, st));
     return TPB200_OK;
 }
 
@@ -502,9 +821,8 @@ extern "C" int tpb200_token_logprobs_backward(const float* grad_logp, const int6
                      rows_range(grad_logp, outer, inner, 1, grad_strides, 4), HostRange{lse, (size_t)rows * 4},
                      HostRange{grad_logits, (size_t)(rows * vocab * dtype_bytes(dtype))});
     const PerToken<long long> lab{(const long long*)labels, label_strides[0], label_strides[1]};
-    TPB_BY_TYPE(dtype, TPB_LAUNCH("score_grad_kernel", score_grad_kernel<T>, dim3((unsigned)rows), 512, 0, st,
-                                  logits_of<T>(logits, inner, vocab, strides), lab, per_token(grad_logp, grad_strides), lse, nullptr, nullptr,
-                                  nullptr, (T*)grad_logits));
+    TPB_BY_TYPE(dtype, return score_grad_run<T>(logits_of<T>(logits, inner, vocab, strides), lab, per_token(grad_logp, grad_strides), lse, nullptr, nullptr,
+                                                nullptr, (T*)grad_logits, rows, st));
     return TPB200_OK;
 }
 
@@ -544,17 +862,18 @@ extern "C" int tpb200_policy_loss(const void* logits, int dtype, int64_t outer, 
         const PolicyTerms terms{per_token(old_logp, old_strides), per_token(advantages, advantage_strides), per_token(weights, weight_strides),
                                 per_token(ref_logp, ref_strides), (float)clip_low, (float)clip_high, (float)kl_coef, (float)grad_scale};
         const PolicyOut out{logp, ratio, kl, (double*)workspace};
-        TPB_BY_TYPE(dtype, TPB_LAUNCH("policy_kernel", policy_kernel<T>, dim3((unsigned)rows), 512, 0, st,
-                                      logits_of<T>(logits, inner, vocab, strides), lab, terms, out, (T*)grad_logits));
+        TPB_BY_TYPE(dtype, rc = (row_run<T, true>(logits_of<T>(logits, inner, vocab, strides), lab, RowLimits{nullptr, 0}, terms, out,
+                                                  ScoreOut{}, (T*)grad_logits, rows, loss, st)));
+        if (rc != TPB200_OK || rows == 1) return rc;     // a single row has written the loss itself
     }
     TPB_LAUNCH("loss_sum_kernel", loss_sum_kernel, dim3(1), 1024, 0, st, (const double*)workspace, (long long)rows, 1.0, loss);
     return TPB200_OK;
 }
 
-// workspace of the preference loss: (m, 1 / s) and the coefficient of every row, the loss of every pair
+// workspace of the preference loss: logp in 64 bits, (reference, 1 / s) and the coefficient of every row, the loss of every pair
 extern "C" size_t tpb200_preference_loss_workspace_bytes(int64_t outer, int64_t inner, int64_t pairs) {
     if (outer < 0 || inner < 0 || pairs < 0) return 0;
-    return (size_t)(outer * inner) * (sizeof(float2) + 8) + (size_t)pairs * sizeof(double);
+    return (size_t)(outer * inner) * (sizeof(double) + sizeof(float2) + sizeof(float)) + (size_t)pairs * sizeof(double);
 }
 
 extern "C" int tpb200_preference_loss(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t vocab,
@@ -580,22 +899,22 @@ extern "C" int tpb200_preference_loss(const void* logits, int dtype, int64_t out
                      HostRange{loss, 4}, HostRange{grad_logits, grad_logits ? (size_t)(rows * vocab * dtype_bytes(dtype)) : 0},
                      HostRange{rewards, (size_t)pairs * 8}, HostRange{logp, (size_t)rows * 4}, HostRange{workspace, need});
     double* part = (double*)workspace;
-    float2* keep = (float2*)(part + pairs);
+    double* exact = part + pairs;
+    float2* keep = (float2*)(exact + rows);
     float* coefs = (float*)(keep + rows);
     const PerToken<long long> lab{(const long long*)labels, label_strides[0], label_strides[1]};
     const RowLimits limits{(const long long*)offsets, 2 * pairs};
     if (rows > 0) {
         if (grad_logits) TPB_LAUNCH("fill_kernel", fill_kernel, dim3((unsigned)ceil_div(rows, 256)), 256, 0, st, coefs, (long long)rows, 0.0f);
-        TPB_BY_TYPE(dtype, TPB_LAUNCH("score_kernel", score_kernel<T>, dim3((unsigned)rows), 512, 0, st,
-                                      logits_of<T>(logits, inner, vocab, strides), lab, limits, logp, nullptr, keep));
+        TPB_BY_TYPE(dtype, rc = score_run<T>(logits_of<T>(logits, inner, vocab, strides), lab, limits, logp, nullptr, keep, exact, rows, st));
+        if (rc != TPB200_OK) return rc;
     }
-    TPB_LAUNCH("pair_kernel", pair_kernel, dim3((unsigned)pairs), 256, 0, st, lab, per_token(ref_logp, ref_strides), (const float*)logp,
+    TPB_LAUNCH("pair_kernel", pair_kernel, dim3((unsigned)pairs), 256, 0, st, lab, per_token(ref_logp, ref_strides), (const double*)exact,
                (const long long*)offsets, (long long)rows, (long long)std::max<int64_t>(inner, 1), (long long)pairs, beta, label_smoothing, grad_scale,
                rewards, part, grad_logits ? coefs : nullptr);
     TPB_LAUNCH("loss_sum_kernel", loss_sum_kernel, dim3(1), 1024, 0, st, (const double*)part, (long long)pairs, 1.0 / (double)pairs, loss);
     if (rows > 0 && grad_logits)
-        TPB_BY_TYPE(dtype, TPB_LAUNCH("score_grad_kernel", score_grad_kernel<T>, dim3((unsigned)rows), 512, 0, st,
-                                      logits_of<T>(logits, inner, vocab, strides), lab, PerToken<float>{nullptr, 0, 0}, (const float*)nullptr,
-                                      (const float2*)keep, (const float*)coefs, (const float*)logp, (T*)grad_logits));
+        TPB_BY_TYPE(dtype, return score_grad_run<T>(logits_of<T>(logits, inner, vocab, strides), lab, PerToken<float>{nullptr, 0, 0}, nullptr, keep, coefs,
+                                                    logp, (T*)grad_logits, rows, st));
     return TPB200_OK;
 }

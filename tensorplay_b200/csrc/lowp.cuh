@@ -67,14 +67,33 @@ template <> struct Elem<__half> {
     }
 };
 
-// 16 bytes of an input that the kernel reads once (past L1) or again soon (kept in L1)
-__device__ __forceinline__ uint4 ld_once16_raw(const void* p) {
+// 16-byte loads and stores with a place in L2's order of eviction.  Streams go first: what is read or written
+// once must not push out what is read again (the logits between two sweeps, the rows of a neighbouring
+// kernel).  Measured on the gradient of [4096,50016] bf16 logits: 5.88 TB/s without, 6.22 TB/s with; on the
+// policy loss, whose second sweep finds its row in L2, 3.97 and 4.97 TB/s of one read and one write.
+__device__ __forceinline__ unsigned long long l2_first() {
+    unsigned long long p;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ unsigned long long l2_last() {
+    unsigned long long p;
+    asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ uint4 ld_policy16_raw(const void* p, unsigned long long policy) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.global.nc.L1::no_allocate.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p), "l"(policy));
     return v;
 }
-#define ld_once16(p) ::tpb::ld_once16_raw(TPB_CKN((p), 16))
-#define st_out16(p, v) (*reinterpret_cast<uint4*>(TPB_CKN((p), 16)) = (v))
+__device__ __forceinline__ void st_stream16_raw(void* p, const uint4& v) {
+    asm volatile("st.global.L1::no_allocate.L2::cache_hint.v4.u32 [%0], {%1,%2,%3,%4}, %5;"
+                 ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "l"(l2_first()) : "memory");
+}
+#define ld_policy16(p, policy) ::tpb::ld_policy16_raw(TPB_CKN((p), 16), (policy))
+#define ld_once16(p) ::tpb::ld_policy16_raw(TPB_CKN((p), 16), ::tpb::l2_first())
+#define st_out16(p, v) ::tpb::st_stream16_raw(TPB_CKN((p), 16), (v))
 
 // Eight consecutive elements, 16-byte aligned: one vector of a 16-bit type, two of float32.
 template <class T>

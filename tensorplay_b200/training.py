@@ -19,6 +19,7 @@ comes from torch's allocator on every call, so that calls on other streams and c
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -41,28 +42,35 @@ def _check_tensor(x, what):
         raise NotImplementedError(f"{what}: tensors of rank {x.dim()} are not supported")
 
 
-def _strides(x, lead, what, name):
-    """(outer, inner) strides of a tensor whose dims beside the row are `lead` = its leading sizes: the
-    last of them is `inner`, the ones before it have to collapse to one."""
-    st = x.stride()
+@functools.lru_cache(maxsize=4096)
+def _collapse(lead, st):
+    """(outer, inner) strides as the ABI takes them for the leading sizes `lead` with strides `st`: the last
+    is `inner`, the ones before it have to collapse to one; None if they do not."""
     if len(lead) == 0:
-        return 0, 0
-    if len(lead) == 1:
-        return 0, st[0]
+        return _lib.pair(0, 0)
     size, step = 1, 0
-    for n, s in zip(reversed(lead[:-1]), reversed(st[:len(lead) - 1])):
+    for n, s in zip(reversed(lead[:-1]), reversed(st[:-1])):
         if n == 1:
             continue
         if size > 1 and s != size * step and 0 not in lead:
-            raise NotImplementedError(f"{what}: the leading dims of {name} do not collapse to one stride (use contiguous())")
+            return None
         if size == 1:
             step = s
         size *= n
-    return step, st[len(lead) - 1]
+    return _lib.pair(step, st[-1])
+
+
+def _strides(x, lead, what, name):
+    got = _collapse(lead, x.stride()[:len(lead)])
+    if got is None:
+        raise NotImplementedError(f"{what}: the leading dims of {name} do not collapse to one stride (use contiguous())")
+    return got
 
 
 def _split(lead):
     """(outer, inner) of the leading sizes."""
+    if len(lead) == 1:
+        return 1, lead[0]
     return (math.prod(lead[:-1]), lead[-1]) if lead else (1, 1)
 
 
@@ -71,7 +79,7 @@ def _row_strides(x, what, name):
         raise ValueError(f"{what}: {name} needs at least one dim")
     if x.stride(-1) != 1 and x.shape[-1] > 1:
         raise NotImplementedError(f"{what}: the last dim of {name} must have unit stride (use contiguous())")
-    return _lib.pair(*_strides(x, x.shape[:-1], what, name))
+    return _strides(x, x.shape[:-1], what, name)
 
 
 def _same(t, like, what, name, shape=None):
@@ -104,7 +112,7 @@ def _token(t, logits, dtype, what, name, broadcast=False):
             t = t.expand(lead)
         except RuntimeError:
             raise ValueError(f"{what}: {name} of shape {tuple(t.shape)} does not broadcast to {tuple(lead)}") from None
-    return t.data_ptr(), _lib.pair(*_strides(t, lead, what, name))
+    return t.data_ptr(), _strides(t, lead, what, name)
 
 
 def _logits(logits, labels, what):
@@ -119,6 +127,11 @@ def _logits(logits, labels, what):
 
 def _scratch(nbytes, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _per_token(lead, device, count):
+    """`count` contiguous float32 outputs of shape `lead` from one allocation."""
+    return torch.empty((count, *lead), dtype=torch.float32, device=device).unbind(0)
 
 
 def _ptr(t):
@@ -162,7 +175,24 @@ def _no_overlap(what, outs, ins):
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)     # torch.cuda.current_stream builds an object: 4 us
+
+
+class _Stay:
+    """The current device is the right one already (torch.cuda.device costs 3 us either way)."""
+
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *_):
+        pass
+
+
+_STAY = _Stay()
+
+
+def _on(device):
+    return _STAY if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 # ---------------------------------------------------------------------------- objectives on logits
@@ -176,9 +206,11 @@ def token_logprobs(logits, labels, *, out=None):
     what = "token_logprobs"
     rows, lab = _logits(logits, labels, what)
     f32 = (logits.shape[:-1], torch.float32)
-    with torch.cuda.device(logits.device):
-        logp, lse = _outputs(what, logits.device, out, [f32, f32])
-        if out is not None:
+    with _on(logits.device):
+        if out is None:
+            logp, lse = _per_token(logits.shape[:-1], logits.device, 2)
+        else:
+            logp, lse = _outputs(what, logits.device, out, [f32, f32])
             _no_overlap(what, (logp, lse), (logits, labels))
         _lib.check(_lib.lib().tpb200_token_logprobs(*rows, *lab, logp.data_ptr(), lse.data_ptr(), _stream(logits.device)))
     return logp, lse
@@ -193,7 +225,7 @@ def token_logprobs_backward(grad_logp, logits, labels, lse, *, out=None):
     _token(lse, logits, torch.float32, what, "lse")
     if not lse.is_contiguous():
         raise ValueError(f"{what}: lse must be contiguous, as token_logprobs returns it")
-    with torch.cuda.device(logits.device):
+    with _on(logits.device):
         g, = _outputs(what, logits.device, out, [(logits.shape, logits.dtype)])
         if out is not None:
             _no_overlap(what, (g,), (logits, labels, grad_logp, lse))
@@ -223,12 +255,17 @@ def policy_loss(logits, labels, old_logp, advantages, weights, ref_logp=None, *,
     device, lead = logits.device, logits.shape[:-1]
     L = _lib.lib()
     f32 = (lead, torch.float32)
-    with torch.cuda.device(device):
-        loss, grad, logp, ratio, kl = _outputs(what, device, out, [((), torch.float32), (logits.shape, logits.dtype) if need_grad else None, f32, f32, f32])
-        if out is not None:
-            _no_overlap(what, (loss, grad, logp, ratio, kl), (logits, labels, old_logp, advantages, weights, ref_logp))
+    with _on(device):
         nbytes = L.tpb200_policy_loss_workspace_bytes(rows[2], rows[3])
-        ws = _scratch(nbytes, device)
+        if out is None:
+            # one allocation for the workspace (8 bytes per token) and what comes back per token
+            ws, _, logp, ratio, kl = _per_token(lead, device, 5)
+            loss = torch.empty((), dtype=torch.float32, device=device)
+            grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if need_grad else None
+        else:
+            loss, grad, logp, ratio, kl = _outputs(what, device, out, [((), torch.float32), (logits.shape, logits.dtype) if need_grad else None, f32, f32, f32])
+            _no_overlap(what, (loss, grad, logp, ratio, kl), (logits, labels, old_logp, advantages, weights, ref_logp))
+            ws = _scratch(nbytes, device)
         _lib.check(L.tpb200_policy_loss(*rows, *lab, *args[0], *args[1], *args[2], *args[3], clip_low, clip_high, kl_coef, grad_scale,
                                         loss.data_ptr(), _ptr(grad), logp.data_ptr(), ratio.data_ptr(), kl.data_ptr(), _ptr(ws), nbytes,
                                         _stream(device)))
@@ -264,7 +301,7 @@ def preference_loss(logits, labels, ref_logp, offsets=None, *, beta=0.1, label_s
     if sequences < 2 or sequences % 2:
         raise ValueError(f"{what}: an even number of sequences is needed (got {sequences})")
     L = _lib.lib()
-    with torch.cuda.device(device):
+    with _on(device):
         loss, grad, rewards, logp = _outputs(what, device, out, [((), torch.float32), (logits.shape, logits.dtype) if need_grad else None,
                                                                  ((sequences,), torch.float32), (logits.shape[:-1], torch.float32)])
         if out is not None:
@@ -336,7 +373,7 @@ def rms_norm(x, weight, eps=1e-6, *, out=None):
         raise TypeError(f"{what}: weight must be a tensor")
     _weight(weight, x, what, "weight")
     strides = _row_strides(x, what, "x")
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         y, rstd = _outputs(what, x.device, out, [(x.shape, x.dtype), (x.shape[:-1], torch.float32)])
         if out is not None:
             _no_overlap(what, (y, rstd), (x, weight))
@@ -366,7 +403,7 @@ def rms_norm_backward(grad_y, x, weight, rstd, *, out=None):
     _rstd(rstd, x, what, "rstd")
     gs, xs = _row_strides(grad_y, what, "grad_y"), _row_strides(x, what, "x")
     L = _lib.lib()
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         gx, gw = _outputs(what, x.device, out, [(x.shape, x.dtype), (weight.shape, x.dtype)])
         if out is not None:
             _no_overlap(what, (gx, gw), (grad_y, x, weight, rstd))
@@ -398,7 +435,7 @@ def block_residual(x, h, post_weight=None, next_weight=None, gate=None, *, scale
     xs, hs = _row_strides(x, what, "x"), _row_strides(h, what, "h")
     f32 = (x.shape[:-1], torch.float32)
     same = (x.shape, x.dtype)
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         outs = _outputs(what, x.device, out, [same, same if next_weight is not None else None, f32 if post_weight is not None else None,
                                               f32 if next_weight is not None else None])
         if out is not None:
@@ -436,7 +473,7 @@ def block_residual_backward(grad_x_out, grad_y, h, x_out, rstd_post, rstd_next, 
         _rstd(rstd_post, h, what, "rstd_post")
     same, row = (h.shape, h.dtype), ((h.shape[-1],), h.dtype)
     L = _lib.lib()
-    with torch.cuda.device(h.device):
+    with _on(h.device):
         outs = _outputs(what, h.device, out, [same, same, row if post_weight is not None else None, row if next_weight is not None else None,
                                               (gate.shape, h.dtype) if gate is not None else None])
         if out is not None:
@@ -460,7 +497,7 @@ def _dropout(x, p, seed, offset, out, what):
     else:
         outer, inner = _split(x.shape[:-1])
         width, strides = x.shape[-1], _row_strides(x, what, "x")
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         y, = _outputs(what, x.device, out, [(x.shape, x.dtype)])
         if out is not None:
             _no_overlap(what, (y,), (x,))

@@ -109,17 +109,18 @@ def test_block_and_dropout_refusals(lib):
 
 def test_strides_of_views():
     from tensorplay_b200 import training as T
+    strides = lambda *a: tuple(T._strides(*a))  # noqa: E731
     x = torch.empty(4, 6, 10)
-    assert T._strides(x, x.shape[:-1], "t", "x") == (60, 10)
-    assert T._strides(x[:, 1:], x[:, 1:].shape[:-1], "t", "x") == (60, 10)
-    assert T._strides(x[0], (6,), "t", "x") == (0, 10)
-    assert T._strides(x[0, 0], (), "t", "x") == (0, 0)
+    assert strides(x, x.shape[:-1], "t", "x") == (60, 10)
+    assert strides(x[:, 1:], x[:, 1:].shape[:-1], "t", "x") == (60, 10)
+    assert strides(x[0], (6,), "t", "x") == (0, 10)
+    assert strides(x[0, 0], (), "t", "x") == (0, 0)
     y = torch.empty(2, 4, 6, 10)
-    assert T._strides(y, y.shape[:-1], "t", "x") == (60, 10)
+    assert strides(y, y.shape[:-1], "t", "x") == (60, 10)
     z = torch.empty(1).expand(2, 4, 6)
-    assert T._strides(z, (2, 4, 6), "t", "x") == (0, 0)
+    assert strides(z, (2, 4, 6), "t", "x") == (0, 0)
     with pytest.raises(NotImplementedError, match="collapse"):
-        T._strides(y.transpose(0, 1), (4, 2, 6), "t", "x")
+        strides(y.transpose(0, 1), (4, 2, 6), "t", "x")
     with pytest.raises(NotImplementedError, match="unit stride"):
         T._row_strides(x.transpose(1, 2), "t", "x")
     assert T._split((2, 3, 5)) == (6, 5) and T._split(()) == (1, 1) and T._split((7,)) == (1, 7)
