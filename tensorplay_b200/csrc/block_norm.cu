@@ -77,18 +77,31 @@ __device__ __forceinline__ void put8(T* p, int u, int tid, int nthr, int width, 
         }
     }
 }
+// Rows that are no whole blocks of the generator (any width that is no multiple of 8): the threads of a row draw
+// the blocks that it touches into shared memory, one byte for eight elements, `base` = the row's first element.
+template <bool WARP>
+__device__ __forceinline__ void draw_row(const DropSpec& d, unsigned long long base, int width, int tid, int nthr, unsigned char* keep) {
+    if (WARP) __syncwarp();      // the row before has been read (a CTA's rows are a barrier apart anyway)
+    const unsigned long long first = base >> 3, last = (base + (unsigned)width - 1) >> 3;
+    for (unsigned long long b = first + tid; b <= last; b += nthr) keep[b - first] = (unsigned char)keep_bits8(b, d);
+    if (WARP) __syncwarp();
+    else __syncthreads();
+}
+// v := dropout(v) for a thread's eight elements of row r
 template <bool VEC>
-__device__ __forceinline__ void factors8(const DropSpec& d, long long r, int u, int tid, int nthr, int width, float* f) {
-    if (d.units == 0) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c) f[c] = 1.0f;
-    } else if (VEC) {
-        drop_factors8((unsigned long long)(r * (width >> 3) + (u * nthr + tid)), d, f);
+__device__ __forceinline__ void drop_row8(const DropSpec& d, long long r, int u, int tid, int nthr, int width, const unsigned char* keep, float* v) {
+    if (VEC) {
+        drop8((unsigned long long)(r * (width >> 3) + (u * nthr + tid)), d, v);
     } else {
+        const int skip = (int)((unsigned long long)(r * width) & 7);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) f[c] = drop_factor1((unsigned long long)(r * width + at<VEC>(u, c, tid, nthr)), d);
+        for (int c = 0; c < 8; ++c) {
+            const int i = at<VEC>(u, c, tid, nthr);
+            if (i < width) v[c] = keep[(skip + i) >> 3] >> ((skip + i) & 7) & 1 ? v[c] * d.factor : 0.0f;
+        }
     }
 }
+__host__ __device__ constexpr int keep_bytes(int width) { return width / 8 + 16; }
 
 // Sum over the threads of a row: a warp, or the CTA (`red` then has 32 slots that the next call must not reuse).
 template <bool WARP>
@@ -101,23 +114,30 @@ __device__ __forceinline__ float row_add(float v, float* red) {
     return warp_add(lane < nw ? red[lane] : 0.0f);
 }
 
+#ifdef TPB200_CHECKED
+template <int NV> constexpr int kForwardCtas = 1;                  // the checker's own function needs 38 registers
+#else
+template <int NV> constexpr int kForwardCtas = NV == 1 ? 2 : 1;    // 32 registers, 64 warps on an SM
+#endif
 template <class T, int NV, bool VEC, bool WARP>
-__global__ void __launch_bounds__(1024)
+__global__ void __launch_bounds__(1024, kForwardCtas<NV>)
 block_forward_kernel(ForwardArgs<T> k) {
+    extern __shared__ unsigned char keep_mem[];      // keep_bytes per row of the CTA, without VEC and with dropout
     __shared__ float red[2][32];
     const int tid = WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x, nthr = WARP ? 32 : (int)blockDim.x;
-    const long long r = WARP ? (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : (long long)blockIdx.x;
+    const unsigned r = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
     if (WARP && r >= k.rows) return;
-    const long long a = r / k.inner, b = r - a * k.inner;
+    const unsigned a = r / (unsigned)k.inner, b = r - a * (unsigned)k.inner;
     const float inv_width = 1.0f / (float)k.width;
     float x[NV][8], h[NV][8];
-    const T* px = k.x.row(a, b);
-#pragma unroll
-    for (int u = 0; u < NV; ++u) fetch8<T, VEC>(px, u, tid, nthr, k.width, x[u]);
-    if (k.h.p) {
-        const T* ph = k.h.row(a, b);
+    const T *px = k.x.row(a, b), *ph = k.h.p ? k.h.row(a, b) : nullptr, *pg = k.gate.p ? k.gate.row(a, b) : nullptr;
+    if (ph) {
 #pragma unroll
         for (int u = 0; u < NV; ++u) fetch8<T, VEC>(ph, u, tid, nthr, k.width, h[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < NV; ++u) fetch8<T, VEC>(px, u, tid, nthr, k.width, x[u]);
+    if (ph) {
         float rstd = 1.0f;
         if (k.post) {
             float s = 0.0f;
@@ -128,28 +148,26 @@ block_forward_kernel(ForwardArgs<T> k) {
             rstd = rsqrtf(row_add<WARP>(s, red[0]) * inv_width + k.eps);
             if (tid == 0) *TPB_CK(&k.rstd_post[r]) = rstd;
         }
-        const T* pg = k.gate.p ? k.gate.row(a, b) : nullptr;
+        unsigned char* keep = keep_mem + (WARP ? (threadIdx.x >> 5) * keep_bytes(k.width) : 0);
+        if (!VEC && k.drop.units) draw_row<WARP>(k.drop, (unsigned long long)r * k.width, k.width, tid, nthr, keep);
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
-            float w[8], f[8];
             if (k.post) {
+                float w[8];
                 fetch8<T, VEC>(k.post, u, tid, nthr, k.width, w);
 #pragma unroll
                 for (int c = 0; c < 8; ++c) h[u][c] = h[u][c] * rstd * w[c];
             }
-            if (k.drop.units) {
-                factors8<VEC>(k.drop, r, u, tid, nthr, k.width, f);
-#pragma unroll
-                for (int c = 0; c < 8; ++c) h[u][c] = f[c] == 0.0f ? 0.0f : h[u][c] * f[c];
-            }
+            if (k.drop.units) drop_row8<VEC>(k.drop, r, u, tid, nthr, k.width, keep, h[u]);
             if (pg) {
-                fetch8<T, VEC>(pg, u, tid, nthr, k.width, w);
+                float g[8];
+                fetch8<T, VEC>(pg, u, tid, nthr, k.width, g);
 #pragma unroll
-                for (int c = 0; c < 8; ++c) h[u][c] *= w[c];
+                for (int c = 0; c < 8; ++c) h[u][c] *= g[c];
             }
 #pragma unroll
             for (int c = 0; c < 8; ++c) x[u][c] = fmaf(k.scale, h[u][c], x[u][c]);
-            put8<T, VEC>(k.x_out + r * k.width, u, tid, nthr, k.width, x[u]);
+            put8<T, VEC>(k.x_out + (long long)r * k.width, u, tid, nthr, k.width, x[u]);
         }
     }
     if (!k.next) return;
@@ -166,7 +184,121 @@ block_forward_kernel(ForwardArgs<T> k) {
         fetch8<T, VEC>(k.next, u, tid, nthr, k.width, w);
 #pragma unroll
         for (int c = 0; c < 8; ++c) w[c] *= x[u][c] * rstd;
-        put8<T, VEC>(k.y + r * k.width, u, tid, nthr, k.width, w);
+        put8<T, VEC>(k.y + (long long)r * k.width, u, tid, nthr, k.width, w);
+    }
+}
+
+// ---------------------------------------------------------------- staged rows ----------------
+// 16-byte aligned rows of up to 8192 elements, one eight-element vector per thread: persistent CTAs, whose threads
+// copy their warp's vectors of the next row into shared memory (cp.async; no barrier over the CTA) while they work
+// on this one, so that a row's reductions over the CTA do not wait for memory.
+constexpr int kStages = 2;
+
+__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)),
+                 "l"(TPB_CKN(src, 16)), "l"(l2_first()) : "memory");
+}
+// One stage.  A warp's 32 vectors of an array are 32 * kVec consecutive 16-byte pieces in memory and in the stage;
+// lane l copies the pieces l, l + 32, so that a float32 row is read in whole sectors too (each lane copying its
+// own 32 bytes took twice the time), and reads its own pieces back.
+template <class T>
+struct Staged {
+    static constexpr int kVec = 8 * sizeof(T) / 16;       // pieces of a thread's vector
+    uint4* warp_at;     // the warp's first piece of array 0
+    int nthr;
+    __device__ __forceinline__ Staged(uint4* mem, int stage, int arrays, int n)
+        : warp_at(mem + (size_t)stage * arrays * kVec * n + (threadIdx.x & ~31u) * kVec), nthr(n) {}
+    __device__ __forceinline__ void fill(int array, const T* row, int width) const {
+        const int lane = threadIdx.x & 31, first = (int)(threadIdx.x & ~31u) * kVec;
+        const uint4* p = reinterpret_cast<const uint4*>(row) + first;
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+            if ((first + j * 32 + lane) * Elem<T>::N < width) copy_async16(warp_at + (size_t)array * kVec * nthr + j * 32 + lane, p + j * 32 + lane);
+    }
+    __device__ __forceinline__ void read(int array, float* f) const {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) Elem<T>::unpack(warp_at[(size_t)array * kVec * nthr + (threadIdx.x & 31) * kVec + j], f + j * Elem<T>::N);
+    }
+    // what the lanes of a warp have copied is there for all of them, or has been read by all of them
+    static __device__ __forceinline__ void sync() {
+        if (kVec > 1) __syncwarp();
+    }
+};
+
+constexpr int kForwardArrays = 3;      // h, x, gate
+template <class T>
+__global__ void __launch_bounds__(1024, kForwardCtas<1>)
+block_forward_staged_kernel(ForwardArgs<T> k) {
+    extern __shared__ __align__(16) uint4 stage_mem[];
+    __shared__ float red[2][2][32];
+    const int tid = threadIdx.x, nthr = blockDim.x, e = tid * 8;
+    const bool mine = e < k.width;
+    const float inv_width = 1.0f / (float)k.width;
+    const unsigned rows = (unsigned)k.rows, step = gridDim.x;
+    int turn = 0;
+    const auto prefetch = [&](unsigned r, int t) {
+        if (r < rows) {
+            const unsigned a = r / (unsigned)k.inner, b = r - a * (unsigned)k.inner;
+            const Staged<T> st(stage_mem, t & 1, kForwardArrays, nthr);
+            Staged<T>::sync();
+            if (k.h.p) st.fill(0, k.h.row(a, b), k.width);
+            st.fill(1, k.x.row(a, b), k.width);
+            if (k.gate.p) st.fill(2, k.gate.row(a, b), k.width);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    prefetch(blockIdx.x, 0);
+    for (unsigned r = blockIdx.x; r < rows; r += step, ++turn) {       // rows + step stays below 2^32
+        prefetch(r + step, turn + 1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        Staged<T>::sync();
+        const Staged<T> st(stage_mem, turn & 1, kForwardArrays, nthr);
+        float* sums = red[turn & 1][0];        // alternates: whoever writes it again has passed a barrier of the row between
+        float v[8], w[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = 0.0f;
+        if (k.h.p) {
+            float rstd = 1.0f;
+            if (mine) st.read(0, v);
+            if (k.post) {
+                float s = 0.0f;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) s = fmaf(v[c], v[c], s);
+                rstd = rsqrtf(row_add<false>(s, sums) * inv_width + k.eps);
+                if (tid == 0) *TPB_CK(&k.rstd_post[r]) = rstd;
+                if (mine) {
+                    load8(k.post + e, w);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) v[c] = v[c] * rstd * w[c];
+                }
+            }
+            if (mine) {
+                if (k.drop.units) drop8((unsigned long long)r * (k.width >> 3) + tid, k.drop, v);
+                if (k.gate.p) {
+                    st.read(2, w);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) v[c] *= w[c];
+                }
+                st.read(1, w);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) v[c] = fmaf(k.scale, v[c], w[c]);
+                store8(k.x_out + (long long)r * k.width + e, v);
+            }
+        } else if (mine) {
+            st.read(1, v);
+        }
+        if (!k.next) continue;
+        float s = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) s = fmaf(v[c], v[c], s);
+        const float rstd = rsqrtf(row_add<false>(s, sums + 32) * inv_width + k.eps);
+        if (tid == 0) *TPB_CK(&k.rstd_next[r]) = rstd;
+        if (mine) {
+            load8(k.next + e, w);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) w[c] *= v[c] * rstd;
+            store8(k.y + (long long)r * k.width + e, w);
+        }
     }
 }
 
@@ -190,6 +322,7 @@ struct BackwardArgs {
 template <class T, int NV, bool VEC, bool WARP>
 __global__ void __launch_bounds__(1024)
 block_backward_kernel(BackwardArgs<T> k) {
+    extern __shared__ unsigned char keep_mem[];      // as in the forward kernel
     __shared__ float red[2][32];
     const int tid = WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x, nthr = WARP ? 32 : (int)blockDim.x;
     const int worker = WARP ? (int)(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) : (int)blockIdx.x;
@@ -257,17 +390,18 @@ block_backward_kernel(BackwardArgs<T> k) {
         for (int u = 0; u < NV; ++u) put8<T, VEC>(k.dx + r * k.width, u, tid, nthr, k.width, t[u]);
         if (k.h.p) {
             const float rstd = k.post ? *TPB_CK(&k.rstd_post[r]) : 1.0f;
+            unsigned char* keep = keep_mem + (WARP ? (threadIdx.x >> 5) * keep_bytes(k.width) : 0);
+            if (!VEC && k.drop.units) draw_row<WARP>(k.drop, (unsigned long long)r * k.width, k.width, tid, nthr, keep);
             float s = 0.0f;
 #pragma unroll
             for (int u = 0; u < NV; ++u) {
-                float w[8], f[8], g[8];
+                float w[8], g[8];
                 if (k.post) fetch8<T, VEC>(k.post, u, tid, nthr, k.width, w);
-                factors8<VEC>(k.drop, r, u, tid, nthr, k.width, f);
+                if (k.drop.units) drop_row8<VEC>(k.drop, r, u, tid, nthr, k.width, keep, t[u]);
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     h[u][c] *= rstd;
-                    f[c] *= k.scale;
-                    t[u][c] *= f[c];                                   // scale * factor * t
+                    t[u][c] *= k.scale;                                // scale * factor * t
                 }
                 if (k.gate.p) {
                     fetch8<T, VEC>(k.gate.row(a, b), u, tid, nthr, k.width, g);
@@ -275,7 +409,7 @@ block_backward_kernel(BackwardArgs<T> k) {
 #pragma unroll
                     for (int c = 0; c < 8; ++c) {
                         const float n = k.post ? h[u][c] * w[c] : h[u][c];
-                        dg[c] = f[c] == 0.0f ? 0.0f : n * t[u][c];
+                        dg[c] = n * t[u][c];
                         acc_gate[u][c] += dg[c];
                         t[u][c] *= g[c];
                     }
@@ -320,30 +454,8 @@ block_backward_kernel(BackwardArgs<T> k) {
 }
 
 // ---------------------------------------------------------------- staged backward ------------
-// The same for 16-byte aligned rows of 513 to 8192 elements, one eight-element vector per thread: each thread
-// copies its own vectors of the next row into shared memory (cp.async, no barrier: nobody else reads them)
-// while it works on this one, so that the row's two reductions over the CTA do not wait for memory.  ARRAYS
-// vectors a row at most: grad_x, grad_y, x_out, h, gate.
-__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)),
-                 "l"(TPB_CKN(src, 16)), "l"(l2_first()) : "memory");
-}
-template <class T>
-struct Staged {
-    static constexpr int kVec = 8 * sizeof(T) / 16;       // 16-byte pieces of a thread's vector
-    uint4* at;          // this thread's first piece of this stage
-    int nthr;
-    __device__ __forceinline__ void fill(int array, const T* p) const {
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) copy_async16(at + (array * kVec + j) * nthr, reinterpret_cast<const uint4*>(p) + j);
-    }
-    __device__ __forceinline__ void read(int array, float* f) const {
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) Elem<T>::unpack(at[(array * kVec + j) * nthr], f + j * Elem<T>::N);
-    }
-};
-
-constexpr int kStages = 2;
+// The same for 16-byte aligned rows of up to 8192 elements; the next row's vectors of grad_x, grad_y, x_out, h and gate
+// arrive while this one is worked on.
 constexpr int kStageArrays = 5;
 
 template <class T, bool SUM_GATE>
@@ -369,38 +481,42 @@ block_backward_staged_kernel(BackwardArgs<T> k) {
     const bool mine = tid * 8 < k.width;
     const int e = tid * 8;
     // the thread's part of both weights lies behind the stages: 16 float32 registers are not to spare
-    const Staged<T> weights{stage_mem + (size_t)(kStages * kStageArrays * Staged<T>::kVec) * nthr + tid, nthr};
-    const auto stage = [&](long long r) {
-        return Staged<T>{stage_mem + (r & 1) * (size_t)(kStageArrays * Staged<T>::kVec) * nthr + tid, nthr};
-    };
+    const Staged<T> weights(stage_mem, kStages, kStageArrays, nthr);
     const auto prefetch = [&](long long r) {
-        if (r < hi && mine) {
-            const long long a = r / k.inner, b = r - a * k.inner;
-            const Staged<T> st = stage(r);
-            if (k.grad_x.p) st.fill(0, k.grad_x.row(a, b) + e);
+        if (r < hi) {
+            const unsigned a = (unsigned)r / (unsigned)k.inner, b = (unsigned)r - a * (unsigned)k.inner;
+            const Staged<T> st(stage_mem, (int)(r & 1), kStageArrays, nthr);
+            Staged<T>::sync();
+            if (k.grad_x.p) st.fill(0, k.grad_x.row(a, b), k.width);
             if (k.next) {
-                st.fill(1, k.grad_y.row(a, b) + e);
-                st.fill(2, k.x_out.row(a, b) + e);
+                st.fill(1, k.grad_y.row(a, b), k.width);
+                st.fill(2, k.x_out.row(a, b), k.width);
             }
-            if (k.h.p) st.fill(3, k.h.row(a, b) + e);
-            if (k.gate.p) st.fill(4, k.gate.row(a, b) + e);
+            if (k.h.p) st.fill(3, k.h.row(a, b), k.width);
+            if (k.gate.p) st.fill(4, k.gate.row(a, b), k.width);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    float acc_post[8], acc_next[8], acc_gate[SUM_GATE ? 8 : 1];
+    // and behind them the gate's running sums
+    float4* gate_sum = reinterpret_cast<float4*>(stage_mem + (size_t)((kStages * kStageArrays + 2) * Staged<T>::kVec) * nthr) + tid;
+    if (SUM_GATE) gate_sum[0] = gate_sum[nthr] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const auto store_gate = [&](auto* dst) {
+        const float4 p = gate_sum[0], q = gate_sum[nthr];
+        const float v[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+        if (mine) store8(dst, v);
+    };
+    float acc_post[8], acc_next[8];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-        acc_post[c] = acc_next[c] = 0.0f;
-        if (SUM_GATE) acc_gate[c] = 0.0f;
-    }
-    if (mine && k.next) weights.fill(0, k.next + e);
-    if (mine && k.post) weights.fill(1, k.post + e);
+    for (int c = 0; c < 8; ++c) acc_post[c] = acc_next[c] = 0.0f;
+    if (k.next) weights.fill(0, k.next, k.width);
+    if (k.post) weights.fill(1, k.post, k.width);
     prefetch(lo);
     for (long long r = lo; r < hi; ++r) {
         prefetch(r + 1);
         const float rstd_next = k.next ? *TPB_CK(&k.rstd_next[r]) : 1.0f, rstd_post = k.post ? *TPB_CK(&k.rstd_post[r]) : 1.0f;
         asm volatile("cp.async.wait_group 1;" ::: "memory");
-        const Staged<T> st = stage(r);
+        Staged<T>::sync();
+        const Staged<T> st(stage_mem, (int)(r & 1), kStageArrays, nthr);
         float t[8], u[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) t[c] = 0.0f;
@@ -437,22 +553,23 @@ block_backward_staged_kernel(BackwardArgs<T> k) {
             float s = 0.0f, hat[8];
             if (mine) {
                 st.read(3, hat);
-                factors8<true>(k.drop, r, 0, tid, nthr, k.width, u);
+                if (k.drop.units) drop8((unsigned long long)(r * (k.width >> 3) + tid), k.drop, t);
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     hat[c] *= rstd_post;
-                    u[c] *= k.scale;
-                    t[c] *= u[c];                                  // scale * factor * t
+                    t[c] *= k.scale;                               // scale * factor * t
                 }
                 float w[8];
                 if (k.post) weights.read(1, w);
                 if (k.gate.p) {
                     float g[8];
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) u[c] = u[c] == 0.0f ? 0.0f : (k.post ? hat[c] * w[c] : hat[c]) * t[c];
+                    for (int c = 0; c < 8; ++c) u[c] = (k.post ? hat[c] * w[c] : hat[c]) * t[c];
                     if (SUM_GATE) {
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) acc_gate[c] += u[c];
+                        float4 q = gate_sum[0];
+                        gate_sum[0] = make_float4(q.x + u[0], q.y + u[1], q.z + u[2], q.w + u[3]);
+                        q = gate_sum[nthr];
+                        gate_sum[nthr] = make_float4(q.x + u[4], q.y + u[5], q.z + u[6], q.w + u[7]);
                     } else {
                         store8(k.dgate + r * k.width + e, u);
                     }
@@ -478,9 +595,8 @@ block_backward_staged_kernel(BackwardArgs<T> k) {
             }
             if (mine) store8(k.dh + r * k.width + e, t);
             if (SUM_GATE && k.groups_per_worker > 0 && (r + 1) % k.group_len == 0) {   // the group is complete
-                if (mine) store8(k.dgate + (r / k.group_len) * k.width + e, acc_gate);
-#pragma unroll
-                for (int c = 0; c < (SUM_GATE ? 8 : 1); ++c) acc_gate[c] = 0.0f;
+                store_gate(k.dgate + (r / k.group_len) * k.width + e);
+                gate_sum[0] = gate_sum[nthr] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
         }
         // `sums` alternates by the row: whoever writes it again has passed a barrier of the row between, which
@@ -489,7 +605,7 @@ block_backward_staged_kernel(BackwardArgs<T> k) {
     if (mine) {
         if (k.post && k.h.p) store8(k.part_post + (long long)worker * k.width + e, acc_post);
         if (k.next) store8(k.part_next + (long long)worker * k.width + e, acc_next);
-        if (SUM_GATE && k.groups_per_worker == 0) store8(k.part_gate + (long long)worker * k.width + e, acc_gate);
+        if (SUM_GATE && k.groups_per_worker == 0) store_gate(k.part_gate + (long long)worker * k.width + e);
     }
 }
 
@@ -533,17 +649,26 @@ inline RowPlan plan_rows(int64_t width, bool vec) {
     return p;
 }
 
-// Rows of the staged kernel: two stages of five arrays fit the shared memory (float32: up to 5 K elements).
-template <class T> inline size_t stage_bytes(int64_t width) { return (size_t)(kStages * kStageArrays + 2) * round_up(ceil_div(width, 8), 32) * 8 * sizeof(T); }
+// Shared memory of the staged kernels: two stages of the arrays; for the backward pass both weights and the gate's
+// sums.  They take rows of up to 8192 elements as long as that fits (backward, float32: up to some 4.5 K elements).
+inline int staged_threads(int64_t width) { return (int)round_up(ceil_div(width, 8), 32); }
+inline size_t backward_bytes(int64_t width, size_t elem, bool sum_gate) {
+    return (size_t)staged_threads(width) * ((kStages * kStageArrays + 2) * 8 * elem + (sum_gate ? 32 : 0));
+}
+// CTAs of a persistent kernel that an SM holds: its threads by registers, 227 KB of shared memory, 32 CTAs.
+// One more than fits would run after the others, with the rows dealt out twice the time.
+inline int resident_ctas(int threads, int most_threads, size_t smem) {
+    const size_t each = (size_t)round_up((long long)(smem + 512 + 1024), 1024);      // static and reserved shared memory
+    return (int)std::max<size_t>(1, std::min<size_t>({32, (size_t)(most_threads / threads), (227 * 1024 + 1024) / each}));
+}
 
 // How the rows are shared out for the backward pass; depends on sizes only, for the workspace query.
 struct Sharing {
     long long groups, group_len, split_len, groups_per_worker;
     int splits, workers;
 };
-inline Sharing share_rows(long long rows, long long groups, int64_t width) {
-    const RowPlan p = plan_rows(width, true);
-    const long long most = p.warp ? 8LL * 4 * sm_count() : (long long)sm_count() * std::max(1, 1024 / p.threads);
+inline Sharing share_rows(long long rows, long long groups, int64_t width, size_t elem, bool sum_gate) {
+    const long long most = (long long)sm_count() * (width <= 8192 ? resident_ctas(staged_threads(width), 1024, backward_bytes(width, elem, sum_gate)) : 1);
     Sharing s{groups, rows / groups, 0, 0, 1, 1};
     if (groups > 1 && groups >= most) {
         s.groups_per_worker = ceil_div(groups, most);
@@ -561,28 +686,41 @@ template <class T, class K>
 bool aligned_row(const RowView<K>& v) { return (((uintptr_t)v.p) & 15) == 0 && (v.s0 * (long long)sizeof(T)) % 16 == 0 && (v.s1 * (long long)sizeof(T)) % 16 == 0; }
 inline bool aligned16(const void* p) { return (((uintptr_t)p) & 15) == 0; }
 
-#define TPB_BLOCK_LAUNCH(KERNEL, T, plan, grid, st, args)                                                                       \
+#define TPB_BLOCK_LAUNCH(KERNEL, T, plan, grid, smem, st, args)                                                                       \
     do {                                                                                                                         \
         if ((plan).warp) {                                                                                                       \
-            if ((plan).vec) { if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, true, true>), grid, (plan).threads, 0, st, args);    \
-                              else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, true, true>), grid, (plan).threads, 0, st, args); }           \
-            else            { if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, false, true>), grid, (plan).threads, 0, st, args);   \
-                              else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, false, true>), grid, (plan).threads, 0, st, args); }          \
+            if ((plan).vec) { if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, true, true>), grid, (plan).threads, (smem), st, args);    \
+                              else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, true, true>), grid, (plan).threads, (smem), st, args); }           \
+            else            { if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, false, true>), grid, (plan).threads, (smem), st, args);   \
+                              else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, false, true>), grid, (plan).threads, (smem), st, args); }          \
         } else {                                                                                                                 \
-            if ((plan).vec) { if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, true, false>), grid, (plan).threads, 0, st, args);   \
-                              else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, true, false>), grid, (plan).threads, 0, st, args); }          \
-            else            { if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, false, false>), grid, (plan).threads, 0, st, args);  \
-                              else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, false, false>), grid, (plan).threads, 0, st, args); }         \
+            if ((plan).vec) { if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, true, false>), grid, (plan).threads, (smem), st, args);   \
+                              else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, true, false>), grid, (plan).threads, (smem), st, args); }          \
+            else            { if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, false, false>), grid, (plan).threads, (smem), st, args);  \
+                              else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, false, false>), grid, (plan).threads, (smem), st, args); }         \
         }                                                                                                                        \
     } while (0)
+
+// shared memory for the kept elements of the CTA's rows, where rows are no whole blocks of the generator
+inline size_t mask_bytes(const RowPlan& p, int width, const DropSpec& d) {
+    return p.vec || d.units == 0 ? 0 : (size_t)keep_bytes(width) * (p.warp ? p.threads / 32 : 1);
+}
 
 template <class T>
 int forward_run(const ForwardArgs<T>& k, cudaStream_t st) {
     const bool vec = k.width % 8 == 0 && aligned_row<T>(k.x) && (!k.h.p || aligned_row<T>(k.h)) && (!k.gate.p || aligned_row<T>(k.gate)) &&
                      aligned16(k.post) && aligned16(k.next) && aligned16(k.x_out) && aligned16(k.y);
+    if (vec && k.width > 256 && k.width <= 8192) {
+        const int threads = staged_threads(k.width);
+        const size_t smem = (size_t)threads * kStages * kForwardArrays * 8 * sizeof(T);
+        TPB_CUDA_OK(cudaFuncSetAttribute(block_forward_staged_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        const long long ctas = std::min<long long>(k.rows, (long long)sm_count() * resident_ctas(threads, 2048, smem));
+        TPB_LAUNCH("block_forward_staged_kernel", block_forward_staged_kernel<T>, dim3((unsigned)ctas), threads, smem, st, k);
+        return TPB200_OK;
+    }
     const RowPlan p = plan_rows(k.width, vec);
     const dim3 grid((unsigned)(p.warp ? ceil_div(k.rows, p.threads / 32) : k.rows));
-    TPB_BLOCK_LAUNCH(block_forward_kernel, T, p, grid, st, k);
+    TPB_BLOCK_LAUNCH(block_forward_kernel, T, p, grid, mask_bytes(p, k.width, k.drop), st, k);
     return TPB200_OK;
 }
 
@@ -593,17 +731,18 @@ int backward_run(const BackwardArgs<T>& k, T* dpost, T* dnext, long long gate_gr
                      aligned16(k.post) && aligned16(k.next) && aligned16(k.dx) && aligned16(k.dh) && aligned16(k.dgate);
     RowPlan p = plan_rows(k.width, vec);
     const dim3 grid((unsigned)(p.warp ? ceil_div(k.workers, p.threads / 32) : k.workers));
-    const size_t smem = stage_bytes<T>(k.width);
-    if (vec && !p.warp && p.nv == 1 && smem <= 220 * 1024) {
+    const size_t smem = backward_bytes(k.width, sizeof(T), k.gate.p && !k.gate_rows);
+    if (vec && k.width <= 8192 && smem <= 226 * 1024) {
+        const int threads = staged_threads(k.width);
         if (k.gate.p && !k.gate_rows) {
             TPB_CUDA_OK(cudaFuncSetAttribute(block_backward_staged_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-            TPB_LAUNCH("block_backward_staged_kernel", (block_backward_staged_kernel<T, true>), grid, p.threads, smem, st, k);
+            TPB_LAUNCH("block_backward_staged_kernel", (block_backward_staged_kernel<T, true>), dim3((unsigned)k.workers), threads, smem, st, k);
         } else {
             TPB_CUDA_OK(cudaFuncSetAttribute(block_backward_staged_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-            TPB_LAUNCH("block_backward_staged_kernel", (block_backward_staged_kernel<T, false>), grid, p.threads, smem, st, k);
+            TPB_LAUNCH("block_backward_staged_kernel", (block_backward_staged_kernel<T, false>), dim3((unsigned)k.workers), threads, smem, st, k);
         }
     } else {
-        TPB_BLOCK_LAUNCH(block_backward_kernel, T, p, grid, st, k);
+        TPB_BLOCK_LAUNCH(block_backward_kernel, T, p, grid, mask_bytes(p, k.width, k.drop), st, k);
     }
     const bool sum_gate = k.gate.p && !k.gate_rows && k.groups_per_worker == 0;
     if (!dpost && !dnext && !sum_gate) return TPB200_OK;
@@ -719,7 +858,7 @@ extern "C" int tpb200_rms_norm(const void* x, int dtype, int64_t outer, int64_t 
     [[maybe_unused]] const int64_t e = dtype_bytes(dtype), n = outer * inner;
     TPB_CHECK_RANGES(st, rows_range(x, outer, inner, width, strides, e), HostRange{weight, (size_t)(width * e)}, HostRange{y, (size_t)(n * width * e)},
                      HostRange{rstd, (size_t)n * 4});
-    const DropSpec none{0, 0, 0, 1.0f};
+    const DropSpec none{0, 0, 0, 0, 1.0f};
     if (dtype == TPB200_F32) return forward_call<float>(x, strides, nullptr, nullptr, nullptr, nullptr, nullptr, weight, outer, inner, width, 1.0, eps, none, nullptr, y, nullptr, rstd, st);
     if (dtype == TPB200_BF16) return forward_call<__nv_bfloat16>(x, strides, nullptr, nullptr, nullptr, nullptr, nullptr, weight, outer, inner, width, 1.0, eps, none, nullptr, y, nullptr, rstd, st);
     return forward_call<__half>(x, strides, nullptr, nullptr, nullptr, nullptr, nullptr, weight, outer, inner, width, 1.0, eps, none, nullptr, y, nullptr, rstd, st);
@@ -751,8 +890,10 @@ extern "C" int tpb200_block_residual(const void* x, const int64_t* x_strides, co
 extern "C" size_t tpb200_block_residual_backward_workspace_bytes(int64_t outer, int64_t inner, int64_t width, int has_post, int has_next,
                                                                  int gate_kind) {
     if (outer <= 0 || inner <= 0 || width <= 0 || outer > 0x7fffffffLL || inner > 0x7fffffffLL || outer * inner > 0x7fffffffLL || width > kMaxWidth) return 0;
-    const Sharing s = share_rows(outer * inner, gate_groups_of(gate_kind, outer), width);
-    return block_workspace(nullptr, s, width, has_post != 0, has_next != 0, gate_kind == TPB200_GATE_VECTOR || gate_kind == TPB200_GATE_SEQUENCE).bytes;
+    // the element type is not known here: the workers of the smallest take the most
+    const bool sum_gate = gate_kind == TPB200_GATE_VECTOR || gate_kind == TPB200_GATE_SEQUENCE;
+    const Sharing s = share_rows(outer * inner, gate_groups_of(gate_kind, outer), width, 2, sum_gate);
+    return block_workspace(nullptr, s, width, has_post != 0, has_next != 0, sum_gate).bytes;
 }
 
 extern "C" int tpb200_block_residual_backward(const void* grad_x_out, const int64_t* grad_x_strides, const void* grad_y,
@@ -780,7 +921,7 @@ extern "C" int tpb200_block_residual_backward(const void* grad_x_out, const int6
     if (!grad_x || (grad_x_out && !grad_x_strides) || (next_weight && (!grad_y || !grad_y_strides || !x_out || !x_out_strides || !rstd_next || !grad_next)) ||
         (h && (!h_strides || !grad_h)) || (h && post_weight && (!rstd_post || !grad_post)) || (gated && (!gate || !gate_strides || !grad_gate)))
         return fail(TPB200_ERR_INVALID, "block_residual_backward: NULL pointer argument");
-    c.share = share_rows(n, gated ? gate_groups_of(gate_kind, outer) : 1, width);
+    c.share = share_rows(n, gated ? gate_groups_of(gate_kind, outer) : 1, width, (size_t)e, gated && gate_kind != TPB200_GATE_ELEMENT);
     c.ws = block_workspace(workspace, c.share, width, h && post_weight, next_weight != nullptr, gated && gate_kind != TPB200_GATE_ELEMENT);
     if (c.ws.bytes > 0 && (!workspace || workspace_bytes < c.ws.bytes))
         return fail(TPB200_ERR_WORKSPACE, "block_residual_backward: workspace missing or too small (%zu of %zu bytes)", workspace_bytes, c.ws.bytes);

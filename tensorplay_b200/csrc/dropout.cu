@@ -10,23 +10,31 @@
 
 namespace tpb {
 
-// `n` elements one after the other on both sides, 16-byte aligned: a block of the generator per step.
+// `n` elements one after the other on both sides, 16-byte aligned: a block of the generator per step.  With 32
+// registers, and so 64 warps on an SM, [16384,8192] takes 104.8 us in bfloat16 (5.1 TB/s: the generator's ten rounds are
+// some sixty integer instructions for eight elements) and 172 us in float32 (6.2 TB/s); with 44 registers 118.9 and
+// 176; two vectors in flight per thread gain nothing on top.
+#ifdef TPB200_CHECKED
+constexpr int kDropCtas = 6;     // the checker's own function needs 38 registers
+#else
+constexpr int kDropCtas = 8;
+#endif
 template <class T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, kDropCtas)
 dropout_flat_kernel(const T* __restrict__ x, T* __restrict__ y, long long n, DropSpec d) {
-    const long long blocks = n >> 3;
-    for (long long b = (long long)blockIdx.x * blockDim.x + threadIdx.x; b < blocks; b += (long long)gridDim.x * blockDim.x) {
-        float v[8], f[8];
+    const long long blocks = n >> 3, step = (long long)gridDim.x * blockDim.x;
+    for (long long b = (long long)blockIdx.x * blockDim.x + threadIdx.x; b < blocks; b += step) {
+        float v[8];
         load8(x + 8 * b, v);
-        drop_factors8((unsigned long long)b, d, f);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) v[c] = f[c] == 0.0f ? 0.0f : v[c] * f[c];   // a dropped NaN or infinity is 0
+        if (d.units) drop8((unsigned long long)b, d, v);
         store8(y + 8 * b, v);
     }
-    if (blockIdx.x == 0 && threadIdx.x < (unsigned)(n & 7)) {
-        const long long i = (blocks << 3) + threadIdx.x;
-        const float f = drop_factor1((unsigned long long)i, d);
-        *TPB_CK(&y[i]) = Elem<T>::put(f == 0.0f ? 0.0f : Elem<T>::get(*TPB_CK(&x[i])) * f);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && (n & 7)) {
+        const unsigned keep = d.units ? keep_bits8((unsigned long long)blocks, d) : 0xffu;
+        for (int c = 0; c < (int)(n & 7); ++c) {
+            const long long i = (blocks << 3) + c;
+            *TPB_CK(&y[i]) = Elem<T>::put(keep >> c & 1 ? Elem<T>::get(*TPB_CK(&x[i])) * d.factor : 0.0f);
+        }
     }
 }
 
@@ -37,14 +45,13 @@ dropout_rows_kernel(const T* __restrict__ x, T* __restrict__ y, long long n, lon
                     long long s0, long long s1, DropSpec d) {
     const long long blocks = (n + 7) >> 3;
     for (long long b = (long long)blockIdx.x * blockDim.x + threadIdx.x; b < blocks; b += (long long)gridDim.x * blockDim.x) {
-        float f[8];
-        drop_factors8((unsigned long long)b, d, f);
+        const unsigned keep = d.units ? keep_bits8((unsigned long long)b, d) : 0xffu;
         long long r = (b << 3) / width, c = (b << 3) - r * width;
         long long o = r / inner, q = r - o * inner;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const long long i = (b << 3) + e;
-            if (i < n) *TPB_CK(&y[i]) = Elem<T>::put(f[e] == 0.0f ? 0.0f : Elem<T>::get(*TPB_CK(&x[o * s0 + q * s1 + c])) * f[e]);
+            if (i < n) *TPB_CK(&y[i]) = Elem<T>::put(keep >> e & 1 ? Elem<T>::get(*TPB_CK(&x[o * s0 + q * s1 + c])) * d.factor : 0.0f);
             if (++c == width) {
                 c = 0;
                 if (++q == inner) { q = 0; ++o; }
@@ -58,7 +65,7 @@ int dropout_run(const void* x, long long outer, long long inner, long long width
                 void* y, cudaStream_t st) {
     const long long n = outer * inner * width;
     const bool flat = (inner == 1 || s1 == width) && (outer == 1 || s0 == inner * width) && (((uintptr_t)x | (uintptr_t)y) & 15) == 0;
-    const long long ctas = std::max(1LL, std::min(ceil_div(ceil_div(n, 8), 256), 16LL * sm_count()));
+    const long long ctas = std::max(1LL, std::min(ceil_div(ceil_div(n, 8), 256), 64LL * sm_count()));
     const dim3 grid((unsigned)ctas);
     if (flat) TPB_LAUNCH("dropout_flat_kernel", dropout_flat_kernel<T>, grid, 256, 0, st, (const T*)x, (T*)y, n, d);
     else TPB_LAUNCH("dropout_rows_kernel", dropout_rows_kernel<T>, grid, 256, 0, st, (const T*)x, (T*)y, n, inner, width, s0, s1, d);

@@ -16,6 +16,7 @@ namespace tpb {
 struct DropSpec {
     unsigned long long seed, offset;
     unsigned units;   // 0: nothing is dropped (no bits are drawn), 65536: everything is
+    unsigned above;   // units * 2^16 - 1: an element is kept iff its bits, shifted to the top of a word, are above it
     float factor;     // of a kept element: 65536 / (65536 - units)
 };
 
@@ -35,23 +36,26 @@ __device__ __forceinline__ uint4 philox_block(unsigned long long index, const Dr
     return make_uint4(c0, c1, c2, c3);
 }
 
-// factors (0 or d.factor) of the eight elements 8 * index .. 8 * index + 7
-__device__ __forceinline__ void drop_factors8(unsigned long long index, const DropSpec& d, float* f) {
+// the eight elements 8 * index .. 8 * index + 7: dropped ones (NaN and infinity too) become 0, kept ones are
+// multiplied by the factor
+__device__ __forceinline__ void drop8(unsigned long long index, const DropSpec& d, float* v) {
     const uint4 w = philox_block(index, d);
-    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        f[2 * j] = (v[j] & 0xffffu) >= d.units ? d.factor : 0.0f;
-        f[2 * j + 1] = (v[j] >> 16) >= d.units ? d.factor : 0.0f;
+        v[2 * j] = (u[j] << 16) > d.above ? v[2 * j] * d.factor : 0.0f;
+        v[2 * j + 1] = u[j] > d.above ? v[2 * j + 1] * d.factor : 0.0f;     // the lower half cannot decide
     }
 }
 
-// factor of one element
-__device__ __forceinline__ float drop_factor1(unsigned long long i, const DropSpec& d) {
-    const uint4 w = philox_block(i >> 3, d);
-    const int j = (int)(i & 7) >> 1;
-    const uint32_t v = j == 0 ? w.x : (j == 1 ? w.y : (j == 2 ? w.z : w.w));
-    return ((i & 1) ? v >> 16 : v & 0xffffu) >= d.units ? d.factor : 0.0f;
+// which of those eight are kept, one bit each
+__device__ __forceinline__ unsigned keep_bits8(unsigned long long index, const DropSpec& d) {
+    const uint4 w = philox_block(index, d);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    unsigned bits = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bits |= ((u[j] << 16) > d.above ? 1u : 0u) << (2 * j) | (u[j] > d.above ? 2u : 0u) << (2 * j);
+    return bits;
 }
 
 // p in [0, 1] -> units and factor; false if p is not a probability
@@ -60,6 +64,7 @@ inline bool make_drop(double p, unsigned long long seed, unsigned long long offs
     d->seed = seed;
     d->offset = offset;
     d->units = (unsigned)(p * 65536.0 + 0.5);
+    d->above = (unsigned)(((unsigned long long)d->units << 16) - 1);
     d->factor = d->units >= 65536u ? 0.0f : (float)(65536.0 / (double)(65536u - d->units));
     return true;
 }
