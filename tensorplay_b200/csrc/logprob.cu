@@ -459,10 +459,27 @@ __device__ __forceinline__ void grad_part(const T* p, T* o, const Part<T>& part,
     }
 }
 
+// The mean of up to kFewPairs losses by one warp; a CTA of the gradient's kernel does it beside its rows.
+constexpr int kFewPairs = 4096;
+struct PairSum {
+    const double* part;   // NULL: nothing to add up
+    int n;
+    float* loss;
+    __device__ __forceinline__ void run() const {
+        if (!part || threadIdx.x >= 32) return;
+        double s = 0.0;
+        for (int i = threadIdx.x; i < n; i += 32) s += *TPB_CK(&part[i]);
+        s = warp_add(s);
+        if (threadIdx.x == 0) *TPB_CK(loss) = (float)(s / (double)n);
+    }
+};
+__global__ void __launch_bounds__(32) pair_sum_kernel(PairSum sum) { sum.run(); }
+
 struct ScoreOut {
     float *logp, *lse;   // all but logp may be NULL
     float2* keep;        // (reference, 1 / s)
     double* exact;       // logp before it is rounded
+    float* coef;         // set to zero: rows of no sequence keep that
 };
 
 // (sum, reference) pairs of the lanes as one
@@ -523,6 +540,7 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
                 if (score.lse) *TPB_CK(&score.lse[r]) = 0.0f;
                 if (score.keep) *TPB_CK(&score.keep[r]) = make_float2(0.0f, 0.0f);
                 if (score.exact) *TPB_CK(&score.exact[r]) = 0.0;
+                if (score.coef) *TPB_CK(&score.coef[r]) = 0.0f;
             }
         }
         if (POLICY && o) zero_part(o, Part<T>(o, in.vocab, rank, C), in.vocab, rank, C);
@@ -599,6 +617,7 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
             if (score.lse) *TPB_CK(&score.lse[r]) = (float)norm;
             if (score.keep) *TPB_CK(&score.keep[r]) = make_float2(m, 1.0f / s);
             if (score.exact) *TPB_CK(&score.exact[r]) = logp;
+            if (score.coef) *TPB_CK(&score.coef[r]) = 0.0f;
         }
     }
     if (!POLICY || !o) return;
@@ -613,7 +632,8 @@ template <class T>
 __global__ void __launch_bounds__(kRowThreads, kRowCtas)
 score_grad_kernel(Logits<T> in, PerToken<long long> labels, PerToken<float> grad_logp, const float* __restrict__ lse,
                   const float2* __restrict__ keep, const float* __restrict__ coefs, const float* __restrict__ logp, T* __restrict__ out, unsigned rows,
-                  int C) {
+                  int C, PairSum sum) {
+    if (blockIdx.x == 0) sum.run();
     // with saved statistics the rows go backwards: the last ones that the sums read are still in L2
     unsigned r = blockIdx.x / (unsigned)C;
     const int rank = (int)(blockIdx.x - r * (unsigned)C);
@@ -716,11 +736,6 @@ pair_kernel(PerToken<long long> labels, PerToken<float> ref, const double* __res
         for (long long r = lo[j] + threadIdx.x; r < hi[j]; r += blockDim.x) *TPB_CK(&coefs[r]) = (float)(j == 0 ? slope : -slope);
 }
 
-__global__ void __launch_bounds__(256) fill_kernel(float* __restrict__ p, long long n, float v) {
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i < n) *TPB_CK(&p[i]) = v;
-}
-
 // ---------------------------------------------------------------- host side -------------------
 template <class T>
 Logits<T> logits_of(const void* x, int64_t inner, int64_t vocab, const int64_t* strides) {
@@ -739,8 +754,9 @@ inline PerToken<float> per_token(const float* p, const int64_t* strides) {
 
 // Threads of a CTA and CTAs per row.  Short rows get as many threads as they have pairs of vectors.  More than one
 // CTA per row: with a second sweep, so that the rows in flight (four CTAs on every SM) take at most 60 MB, half
-// of L2; and while the rows alone do not fill the GPU and a CTA still has two vectors per thread.  [1024,151936] bf16,
-// C = 1, 2, 3, 4, 6: 4.10, 4.38, 4.46, 4.33, 3.94 TB/s; f32: 4.12, 4.20, 4.44, 4.44, 4.83.
+// of L2; and while all CTAs fit the GPU at once and a CTA still has a vector per thread.  Policy loss on [1024,151936],
+// bf16, C = 1, 2, 3, 4, 6: 4.10, 4.38, 4.46, 4.33, 3.94 TB/s; f32: 4.12, 4.20, 4.44, 4.44, 4.83.  Scores of [256,151936] f32,
+// C = 1, 2 (512 CTAs of 592), 3, 4: 34.6, 28.7, 34.5, 32.2 us; of [1,151936] bf16, C = 1, 4, 8: 11.0, 6.1, 4.8 us.
 struct RowShape { int threads, C; };
 inline RowShape row_shape(int64_t rows, int64_t vocab, int64_t elem, bool twice) {
     const int64_t vectors = vocab * elem / 16, room = 4LL * sm_count();
@@ -748,7 +764,9 @@ inline RowShape row_shape(int64_t rows, int64_t vocab, int64_t elem, bool twice)
     if (s.threads < kRowThreads) return s;
     int64_t C = 1;
     if (twice) C = std::min<int64_t>(kRowCluster, ceil_div(std::min(rows, room) * vocab * elem, 60LL << 20));
-    while (C < kRowCluster && rows * C < room && vectors >= (C + 1) * 2 * kRowThreads) ++C;
+    while (C < kRowCluster && rows * (C + 1) <= room && vectors >= (C + 1) * kRowThreads) ++C;
+    int forced = 0;      // experiment and test switch: that many CTAs per row
+    if (env_int("TPB200_ROW_CTAS", &forced) && forced >= 1 && forced <= kRowCluster) C = forced;
     if (rows * C > 0x7fffffffLL) C = 1;
     s.C = (int)C;
     return s;
@@ -764,15 +782,15 @@ int row_run(const Logits<T>& in, const PerToken<long long>& lab, const RowLimits
 }
 template <class T>
 int score_run(const Logits<T>& in, const PerToken<long long>& lab, const RowLimits& limits, float* logp, float* lse, float2* keep,
-              double* exact, int64_t rows, cudaStream_t st) {
-    return row_run<T, false>(in, lab, limits, PolicyTerms{}, PolicyOut{}, ScoreOut{logp, lse, keep, exact}, (T*)nullptr, rows, nullptr, st);
+              double* exact, float* coef, int64_t rows, cudaStream_t st) {
+    return row_run<T, false>(in, lab, limits, PolicyTerms{}, PolicyOut{}, ScoreOut{logp, lse, keep, exact, coef}, (T*)nullptr, rows, nullptr, st);
 }
 template <class T>
 int score_grad_run(const Logits<T>& in, const PerToken<long long>& lab, const PerToken<float>& grad_logp, const float* lse, const float2* keep,
-                   const float* coefs, const float* logp, T* out, int64_t rows, cudaStream_t st) {
+                   const float* coefs, const float* logp, T* out, int64_t rows, const PairSum& sum, cudaStream_t st) {
     const RowShape s = row_shape(rows, in.vocab, sizeof(T), false);
     TPB_LAUNCH("score_grad_kernel", score_grad_kernel<T>, dim3((unsigned)(rows * s.C)), s.threads, 0, st, in, lab, grad_logp, lse, keep, coefs, logp, out,
-               (unsigned)rows, s.C);
+               (unsigned)rows, s.C, sum);
     return TPB200_OK;
 }
 
@@ -803,7 +821,7 @@ extern "C" int tpb200_token_logprobs(const void* logits, int dtype, int64_t oute
     TPB_CHECK_RANGES(st, rows_range(logits, outer, inner, vocab, strides, dtype_bytes(dtype)), rows_range(labels, outer, inner, 1, label_strides, 8),
                      HostRange{logp, (size_t)rows * 4}, HostRange{lse, (size_t)rows * 4});
     const PerToken<long long> lab{(const long long*)labels, label_strides[0], label_strides[1]};
-    TPB_BY_TYPE(dtype, return score_run<T>(logits_of<T>(logits, inner, vocab, strides), lab, RowLimits{nullptr, 0}, logp, lse, nullptr, nullptr, rows, st));
+    TPB_BY_TYPE(dtype, return score_run<T>(logits_of<T>(logits, inner, vocab, strides), lab, RowLimits{nullptr, 0}, logp, lse, nullptr, nullptr, nullptr, rows, st));
     return TPB200_OK;
 }
 
@@ -822,7 +840,7 @@ extern "C" int tpb200_token_logprobs_backward(const float* grad_logp, const int6
                      HostRange{grad_logits, (size_t)(rows * vocab * dtype_bytes(dtype))});
     const PerToken<long long> lab{(const long long*)labels, label_strides[0], label_strides[1]};
     TPB_BY_TYPE(dtype, return score_grad_run<T>(logits_of<T>(logits, inner, vocab, strides), lab, per_token(grad_logp, grad_strides), lse, nullptr, nullptr,
-                                                nullptr, (T*)grad_logits, rows, st));
+                                                nullptr, (T*)grad_logits, rows, PairSum{}, st));
     return TPB200_OK;
 }
 
@@ -905,16 +923,18 @@ extern "C" int tpb200_preference_loss(const void* logits, int dtype, int64_t out
     const PerToken<long long> lab{(const long long*)labels, label_strides[0], label_strides[1]};
     const RowLimits limits{(const long long*)offsets, 2 * pairs};
     if (rows > 0) {
-        if (grad_logits) TPB_LAUNCH("fill_kernel", fill_kernel, dim3((unsigned)ceil_div(rows, 256)), 256, 0, st, coefs, (long long)rows, 0.0f);
-        TPB_BY_TYPE(dtype, rc = score_run<T>(logits_of<T>(logits, inner, vocab, strides), lab, limits, logp, nullptr, keep, exact, rows, st));
+        TPB_BY_TYPE(dtype, rc = score_run<T>(logits_of<T>(logits, inner, vocab, strides), lab, limits, logp, nullptr, keep, exact, grad_logits ? coefs : nullptr, rows, st));
         if (rc != TPB200_OK) return rc;
     }
     TPB_LAUNCH("pair_kernel", pair_kernel, dim3((unsigned)pairs), 256, 0, st, lab, per_token(ref_logp, ref_strides), (const double*)exact,
                (const long long*)offsets, (long long)rows, (long long)std::max<int64_t>(inner, 1), (long long)pairs, beta, label_smoothing, grad_scale,
                rewards, part, grad_logits ? coefs : nullptr);
-    TPB_LAUNCH("loss_sum_kernel", loss_sum_kernel, dim3(1), 1024, 0, st, (const double*)part, (long long)pairs, 1.0 / (double)pairs, loss);
+    const bool few = pairs <= kFewPairs, beside = few && rows > 0 && grad_logits;
+    const PairSum sum{few ? part : nullptr, few ? (int)pairs : 0, loss};
+    if (!few) TPB_LAUNCH("loss_sum_kernel", loss_sum_kernel, dim3(1), 1024, 0, st, (const double*)part, (long long)pairs, 1.0 / (double)pairs, loss);
+    else if (!beside) TPB_LAUNCH("pair_sum_kernel", pair_sum_kernel, dim3(1), 32, 0, st, sum);
     if (rows > 0 && grad_logits)
         TPB_BY_TYPE(dtype, return score_grad_run<T>(logits_of<T>(logits, inner, vocab, strides), lab, PerToken<float>{nullptr, 0, 0}, nullptr, keep, coefs,
-                                                    logp, (T*)grad_logits, rows, st));
+                                                    logp, (T*)grad_logits, rows, beside ? sum : PairSum{}, st));
     return TPB200_OK;
 }

@@ -125,6 +125,15 @@ def _logits(logits, labels, what):
     return rows, _token(labels, logits, torch.int64, what, "labels")
 
 
+def _new(shape, dtype, like):
+    """A new contiguous tensor on the device of `like`; empty_like takes half the time of empty."""
+    if dtype == like.dtype:
+        if shape == like.shape and like.is_contiguous():
+            return torch.empty_like(like)
+        return like.new_empty(shape)
+    return like.new_empty(shape, dtype=dtype)
+
+
 def _scratch(nbytes, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
@@ -138,10 +147,11 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _outputs(what, device, out, specs):
+def _outputs(what, like, out, specs):
     """New contiguous outputs, or the ones of `out` after a check; specs: (shape, dtype) or None each."""
     if out is None:
-        return [None if s is None else torch.empty(s[0], dtype=s[1], device=device) for s in specs]
+        return [None if s is None else _new(s[0], s[1], like) for s in specs]
+    device = like.device
     if not isinstance(out, (tuple, list)) or len(out) != len(specs):
         raise ValueError(f"{what}: out must hold {len(specs)} tensors")
     for t, s in zip(out, specs):
@@ -210,7 +220,7 @@ def token_logprobs(logits, labels, *, out=None):
         if out is None:
             logp, lse = _per_token(logits.shape[:-1], logits.device, 2)
         else:
-            logp, lse = _outputs(what, logits.device, out, [f32, f32])
+            logp, lse = _outputs(what, logits, out, [f32, f32])
             _no_overlap(what, (logp, lse), (logits, labels))
         _lib.check(_lib.lib().tpb200_token_logprobs(*rows, *lab, logp.data_ptr(), lse.data_ptr(), _stream(logits.device)))
     return logp, lse
@@ -226,7 +236,7 @@ def token_logprobs_backward(grad_logp, logits, labels, lse, *, out=None):
     if not lse.is_contiguous():
         raise ValueError(f"{what}: lse must be contiguous, as token_logprobs returns it")
     with _on(logits.device):
-        g, = _outputs(what, logits.device, out, [(logits.shape, logits.dtype)])
+        g, = _outputs(what, logits, out, [(logits.shape, logits.dtype)])
         if out is not None:
             _no_overlap(what, (g,), (logits, labels, grad_logp, lse))
         _lib.check(_lib.lib().tpb200_token_logprobs_backward(*grad, *rows, *lab, lse.data_ptr(), g.data_ptr(), _stream(logits.device)))
@@ -260,10 +270,10 @@ def policy_loss(logits, labels, old_logp, advantages, weights, ref_logp=None, *,
         if out is None:
             # one allocation for the workspace (8 bytes per token) and what comes back per token
             ws, _, logp, ratio, kl = _per_token(lead, device, 5)
-            loss = torch.empty((), dtype=torch.float32, device=device)
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if need_grad else None
+            loss = _new((), torch.float32, ws)
+            grad = _new(logits.shape, logits.dtype, logits) if need_grad else None
         else:
-            loss, grad, logp, ratio, kl = _outputs(what, device, out, [((), torch.float32), (logits.shape, logits.dtype) if need_grad else None, f32, f32, f32])
+            loss, grad, logp, ratio, kl = _outputs(what, logits, out, [((), torch.float32), (logits.shape, logits.dtype) if need_grad else None, f32, f32, f32])
             _no_overlap(what, (loss, grad, logp, ratio, kl), (logits, labels, old_logp, advantages, weights, ref_logp))
             ws = _scratch(nbytes, device)
         _lib.check(L.tpb200_policy_loss(*rows, *lab, *args[0], *args[1], *args[2], *args[3], clip_low, clip_high, kl_coef, grad_scale,
@@ -302,7 +312,7 @@ def preference_loss(logits, labels, ref_logp, offsets=None, *, beta=0.1, label_s
         raise ValueError(f"{what}: an even number of sequences is needed (got {sequences})")
     L = _lib.lib()
     with _on(device):
-        loss, grad, rewards, logp = _outputs(what, device, out, [((), torch.float32), (logits.shape, logits.dtype) if need_grad else None,
+        loss, grad, rewards, logp = _outputs(what, logits, out, [((), torch.float32), (logits.shape, logits.dtype) if need_grad else None,
                                                                  ((sequences,), torch.float32), (logits.shape[:-1], torch.float32)])
         if out is not None:
             _no_overlap(what, (loss, grad, rewards, logp), (logits, labels, ref_logp, offsets))
@@ -374,7 +384,7 @@ def rms_norm(x, weight, eps=1e-6, *, out=None):
     _weight(weight, x, what, "weight")
     strides = _row_strides(x, what, "x")
     with _on(x.device):
-        y, rstd = _outputs(what, x.device, out, [(x.shape, x.dtype), (x.shape[:-1], torch.float32)])
+        y, rstd = _outputs(what, x, out, [(x.shape, x.dtype), (x.shape[:-1], torch.float32)])
         if out is not None:
             _no_overlap(what, (y, rstd), (x, weight))
         _lib.check(_lib.lib().tpb200_rms_norm(x.data_ptr(), _TYPES[x.dtype], *size, strides, weight.data_ptr(), eps, y.data_ptr(), rstd.data_ptr(),
@@ -404,7 +414,7 @@ def rms_norm_backward(grad_y, x, weight, rstd, *, out=None):
     gs, xs = _row_strides(grad_y, what, "grad_y"), _row_strides(x, what, "x")
     L = _lib.lib()
     with _on(x.device):
-        gx, gw = _outputs(what, x.device, out, [(x.shape, x.dtype), (weight.shape, x.dtype)])
+        gx, gw = _outputs(what, x, out, [(x.shape, x.dtype), (weight.shape, x.dtype)])
         if out is not None:
             _no_overlap(what, (gx, gw), (grad_y, x, weight, rstd))
         nbytes = L.tpb200_rms_norm_backward_workspace_bytes(*size)
@@ -436,7 +446,7 @@ def block_residual(x, h, post_weight=None, next_weight=None, gate=None, *, scale
     f32 = (x.shape[:-1], torch.float32)
     same = (x.shape, x.dtype)
     with _on(x.device):
-        outs = _outputs(what, x.device, out, [same, same if next_weight is not None else None, f32 if post_weight is not None else None,
+        outs = _outputs(what, x, out, [same, same if next_weight is not None else None, f32 if post_weight is not None else None,
                                               f32 if next_weight is not None else None])
         if out is not None:
             _no_overlap(what, outs, (x, h, post_weight, next_weight, gate))
@@ -474,7 +484,7 @@ def block_residual_backward(grad_x_out, grad_y, h, x_out, rstd_post, rstd_next, 
     same, row = (h.shape, h.dtype), ((h.shape[-1],), h.dtype)
     L = _lib.lib()
     with _on(h.device):
-        outs = _outputs(what, h.device, out, [same, same, row if post_weight is not None else None, row if next_weight is not None else None,
+        outs = _outputs(what, h, out, [same, same, row if post_weight is not None else None, row if next_weight is not None else None,
                                               (gate.shape, h.dtype) if gate is not None else None])
         if out is not None:
             _no_overlap(what, outs, (grad_x_out, grad_y, h, x_out, rstd_post, rstd_next, post_weight, next_weight, gate))
@@ -498,7 +508,7 @@ def _dropout(x, p, seed, offset, out, what):
         outer, inner = _split(x.shape[:-1])
         width, strides = x.shape[-1], _row_strides(x, what, "x")
     with _on(x.device):
-        y, = _outputs(what, x.device, out, [(x.shape, x.dtype)])
+        y, = _outputs(what, x, out, [(x.shape, x.dtype)])
         if out is not None:
             _no_overlap(what, (y,), (x,))
         _lib.check(_lib.lib().tpb200_dropout(x.data_ptr(), _TYPES[x.dtype], outer, inner, width, strides, p, seed, offset, y.data_ptr(), _stream(x.device)))
