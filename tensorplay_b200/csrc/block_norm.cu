@@ -191,7 +191,9 @@ block_forward_kernel(ForwardArgs<T> k) {
 // ---------------------------------------------------------------- staged rows ----------------
 // 16-byte aligned rows of up to 8192 elements, one eight-element vector per thread: persistent CTAs, whose threads
 // copy their warp's vectors of the next row into shared memory (cp.async; no barrier over the CTA) while they work
-// on this one, so that a row's reductions over the CTA do not wait for memory.
+// on this one, so that a row's reductions over the CTA do not wait for memory.  [16384,4096] bf16 with an element gate:
+// 119 us without dropout (5.6 TB/s; a CTA per row and no prefetch took 147), 159 us with it (some sixty integer
+// instructions of the generator for eight elements).
 constexpr int kStages = 2;
 
 __device__ __forceinline__ void copy_async16(void* dst, const void* src) {
@@ -455,7 +457,9 @@ block_backward_kernel(BackwardArgs<T> k) {
 
 // ---------------------------------------------------------------- staged backward ------------
 // The same for 16-byte aligned rows of up to 8192 elements; the next row's vectors of grad_x, grad_y, x_out, h and gate
-// arrive while this one is worked on.
+// arrive while this one is worked on.  [16384,4096] bf16 with an element gate: 240 us without dropout (4.5 TB/s), 265 us
+// with it; bound by latency, since 64 registers and two stages leave two CTAs of 512 threads on an SM.  The kernel
+// above, which loads a row when it comes to it, took some 400 us.
 constexpr int kStageArrays = 5;
 
 template <class T, bool SUM_GATE>
