@@ -373,7 +373,9 @@ int tpb200_dropout(const void* x, int dtype, int64_t outer, int64_t inner, int64
  * y goes by x_out before it is rounded.  Rows of at most 16384 elements.
  * The gate's kind, for the gradient: one row for all rows, one per outer index, or one for every row.
  * The backward call gives the gradients of x, h, both weights and the gate from grad_x_out (NULL: zero)
- * and grad_y; weight and gate gradients are sums over rows, taken in a fixed order.
+ * and grad_y; weight and gate gradients are sums over rows, taken in a fixed order.  It goes by the x_out
+ * that it is given, as that was rounded; the _from_x call takes the forward call's x in its place and forms
+ * x_out from it, h and the gate again, before any rounding, which is what y was computed from.
  * tpb200_rms_norm is y = hat(x) * weight alone.
  */
 #define TPB200_GATE_NONE 0
@@ -391,6 +393,13 @@ int tpb200_block_residual_backward(const void* grad_x_out, const int64_t* grad_x
                                    const float* rstd_next, int dtype, int64_t outer, int64_t inner, int64_t width, double scale,
                                    double p, uint64_t seed, uint64_t offset, void* grad_x, void* grad_h, void* grad_post,
                                    void* grad_next, void* grad_gate, void* workspace, size_t workspace_bytes, void* stream);
+int tpb200_block_residual_backward_from_x(const void* grad_x_out, const int64_t* grad_x_strides, const void* grad_y,
+                                          const int64_t* grad_y_strides, const void* h, const int64_t* h_strides, const void* x,
+                                          const int64_t* x_strides, const void* gate, const int64_t* gate_strides, int gate_kind,
+                                          const void* post_weight, const void* next_weight, const float* rstd_post,
+                                          const float* rstd_next, int dtype, int64_t outer, int64_t inner, int64_t width, double scale,
+                                          double p, uint64_t seed, uint64_t offset, void* grad_x, void* grad_h, void* grad_post,
+                                          void* grad_next, void* grad_gate, void* workspace, size_t workspace_bytes, void* stream);
 size_t tpb200_block_residual_backward_workspace_bytes(int64_t outer, int64_t inner, int64_t width, int has_post, int has_next,
                                                       int gate_kind);
 int tpb200_rms_norm(const void* x, int dtype, int64_t outer, int64_t inner, int64_t width, const int64_t* strides,

@@ -39,7 +39,7 @@ SYMBOLS = [
     "tpb200_reduce_sharded", "tpb200_topk_sharded", "tpb200_strided_copy",
     "tpb200_token_logprobs", "tpb200_token_logprobs_backward", "tpb200_policy_loss", "tpb200_policy_loss_workspace_bytes",
     "tpb200_preference_loss", "tpb200_preference_loss_workspace_bytes", "tpb200_dropout", "tpb200_block_residual",
-    "tpb200_block_residual_backward", "tpb200_block_residual_backward_workspace_bytes", "tpb200_rms_norm",
+    "tpb200_block_residual_backward", "tpb200_block_residual_backward_from_x", "tpb200_block_residual_backward_workspace_bytes", "tpb200_rms_norm",
     "tpb200_rms_norm_backward", "tpb200_rms_norm_backward_workspace_bytes",
 ]
 
@@ -149,8 +149,9 @@ def lib() -> ctypes.CDLL:
     L.tpb200_dropout.argtypes = [vp, i, i64, i64, i64, _I64P, f64, u64, u64, vp, vp]
     L.tpb200_block_residual.restype = i
     L.tpb200_block_residual.argtypes = [*view * 3, vp, vp, i, i64, i64, i64, f64, f64, f64, u64, u64, vp, vp, vp, vp, vp]
-    L.tpb200_block_residual_backward.restype = i
-    L.tpb200_block_residual_backward.argtypes = [*view * 5, i, vp, vp, vp, vp, i, i64, i64, i64, f64, f64, u64, u64, vp, vp, vp, vp, vp, vp, sz, vp]
+    for backward in (L.tpb200_block_residual_backward, L.tpb200_block_residual_backward_from_x):
+        backward.restype = i
+        backward.argtypes = [*view * 5, i, vp, vp, vp, vp, i, i64, i64, i64, f64, f64, u64, u64, vp, vp, vp, vp, vp, vp, sz, vp]
     L.tpb200_block_residual_backward_workspace_bytes.restype = sz
     L.tpb200_block_residual_backward_workspace_bytes.argtypes = [i64, i64, i64, i, i, i]
     L.tpb200_rms_norm.restype = i

@@ -10,7 +10,10 @@
 //     b = d * w_post,  dh = rstd_post * (b - hat(h) * mean(b * hat(h)))
 //     dw_next = sum over rows of g_y * hat(x'),  dw_post = sum over rows of d * hat(h)
 // rms_norm is the part with w_next alone.  All of it is float32 between the loads and the one rounding of
-// each output; y and rstd_next go by the x' before it is rounded.
+// each output; y and rstd_next go by the x' before it is rounded.  The backward pass takes x' from the forward
+// call's x, h and gate again, operation by operation (the same bits), or, where it is given x_out instead, as
+// it was rounded there: dw_next of a 16-bit type is then a second rounding of x' off (bfloat16, [2048,4096]:
+// 2.3e-3 of its norm against 1.6e-3).
 #define TPB_FILE_ID 8
 #include "host_util.h"
 #include "lowp.cuh"
@@ -86,6 +89,11 @@ __device__ __forceinline__ void draw_row(const DropSpec& d, unsigned long long b
     for (unsigned long long b = first + tid; b <= last; b += nthr) keep[b - first] = (unsigned char)keep_bits8(b, d);
     if (WARP) __syncwarp();
     else __syncthreads();
+}
+// v := dropout(v) for eight elements whose bits in `keep` say which stay
+__device__ __forceinline__ void drop_by8(const DropSpec& d, unsigned keep, float* v) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) v[c] = keep >> c & 1 ? v[c] * d.factor : 0.0f;
 }
 // v := dropout(v) for a thread's eight elements of row r
 template <bool VEC>
@@ -307,6 +315,7 @@ block_forward_staged_kernel(ForwardArgs<T> k) {
 template <class T>
 struct BackwardArgs {
     RowView<const T> grad_x, grad_y, h, x_out, gate;   // grad_x.p NULL: zero; grad_y.p / x_out.p go with next
+    int from_x;                        // 1: x_out holds the forward call's x (with h and next)
     const T *post, *next;
     const float *rstd_post, *rstd_next;
     T *dx, *dh, *dgate;                // contiguous; dgate: [groups, width], or all rows (gate_rows)
@@ -365,6 +374,9 @@ block_backward_kernel(BackwardArgs<T> k) {
 #pragma unroll
             for (int u = 0; u < NV; ++u) fetch8<T, VEC>(k.h.row(a, b), u, tid, nthr, k.width, h[u]);
         }
+        unsigned char* keep = keep_mem + (WARP ? (threadIdx.x >> 5) * keep_bytes(k.width) : 0);
+        const float rstd_post = k.post && k.h.p ? *TPB_CK(&k.rstd_post[r]) : 1.0f;
+        if (!VEC && k.h.p && k.drop.units) draw_row<WARP>(k.drop, (unsigned long long)r * k.width, k.width, tid, nthr, keep);
         if (k.next) {
             const float rstd = *TPB_CK(&k.rstd_next[r]);
             float xh[NV][8], g[NV][8], s = 0.0f;
@@ -372,6 +384,24 @@ block_backward_kernel(BackwardArgs<T> k) {
             for (int u = 0; u < NV; ++u) {
                 float w[8];
                 fetch8<T, VEC>(k.x_out.row(a, b), u, tid, nthr, k.width, xh[u]);
+                if (k.from_x) {            // x' before it was rounded, by the forward kernel's operations
+                    float n[8];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) n[c] = h[u][c];
+                    if (k.post) {
+                        fetch8<T, VEC>(k.post, u, tid, nthr, k.width, w);
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) n[c] = n[c] * rstd_post * w[c];
+                    }
+                    if (k.drop.units) drop_row8<VEC>(k.drop, r, u, tid, nthr, k.width, keep, n);
+                    if (k.gate.p) {
+                        fetch8<T, VEC>(k.gate.row(a, b), u, tid, nthr, k.width, w);
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) n[c] *= w[c];
+                    }
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) xh[u][c] = fmaf(k.scale, n[c], xh[u][c]);
+                }
                 fetch8<T, VEC>(k.grad_y.row(a, b), u, tid, nthr, k.width, g[u]);
                 fetch8<T, VEC>(k.next, u, tid, nthr, k.width, w);
 #pragma unroll
@@ -391,9 +421,6 @@ block_backward_kernel(BackwardArgs<T> k) {
 #pragma unroll
         for (int u = 0; u < NV; ++u) put8<T, VEC>(k.dx + r * k.width, u, tid, nthr, k.width, t[u]);
         if (k.h.p) {
-            const float rstd = k.post ? *TPB_CK(&k.rstd_post[r]) : 1.0f;
-            unsigned char* keep = keep_mem + (WARP ? (threadIdx.x >> 5) * keep_bytes(k.width) : 0);
-            if (!VEC && k.drop.units) draw_row<WARP>(k.drop, (unsigned long long)r * k.width, k.width, tid, nthr, keep);
             float s = 0.0f;
 #pragma unroll
             for (int u = 0; u < NV; ++u) {
@@ -402,7 +429,7 @@ block_backward_kernel(BackwardArgs<T> k) {
                 if (k.drop.units) drop_row8<VEC>(k.drop, r, u, tid, nthr, k.width, keep, t[u]);
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
-                    h[u][c] *= rstd;
+                    h[u][c] *= rstd_post;
                     t[u][c] *= k.scale;                                // scale * factor * t
                 }
                 if (k.gate.p) {
@@ -431,7 +458,7 @@ block_backward_kernel(BackwardArgs<T> k) {
 #pragma unroll
                 for (int u = 0; u < NV; ++u)
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) t[u][c] = rstd * (t[u][c] - h[u][c] * m);
+                    for (int c = 0; c < 8; ++c) t[u][c] = rstd_post * (t[u][c] - h[u][c] * m);
             }
 #pragma unroll
             for (int u = 0; u < NV; ++u) put8<T, VEC>(k.dh + r * k.width, u, tid, nthr, k.width, t[u]);
@@ -457,12 +484,13 @@ block_backward_kernel(BackwardArgs<T> k) {
 
 // ---------------------------------------------------------------- staged backward ------------
 // The same for 16-byte aligned rows of up to 8192 elements; the next row's vectors of grad_x, grad_y, x_out, h and gate
-// arrive while this one is worked on.  [16384,4096] bf16 with an element gate: 240 us without dropout (4.5 TB/s), 265 us
-// with it; bound by latency, since 64 registers and two stages leave two CTAs of 512 threads on an SM.  The kernel
+// arrive while this one is worked on.  [16384,4096] bf16 with an element gate: 229 us without dropout (4.7 TB/s), 268 us
+// with it; with FROM_X 257 and 302 us, three more reads of shared memory and x' formed again in front of the row's
+// first sum; bound by latency, since 64 registers and two stages leave two CTAs of 512 threads on an SM.  The kernel
 // above, which loads a row when it comes to it, took some 400 us.
 constexpr int kStageArrays = 5;
 
-template <class T, bool SUM_GATE>
+template <class T, bool SUM_GATE, bool FROM_X>
 __global__ void __launch_bounds__(1024, 1)
 block_backward_staged_kernel(BackwardArgs<T> k) {
     extern __shared__ __align__(16) uint4 stage_mem[];
@@ -518,6 +546,8 @@ block_backward_staged_kernel(BackwardArgs<T> k) {
     for (long long r = lo; r < hi; ++r) {
         prefetch(r + 1);
         const float rstd_next = k.next ? *TPB_CK(&k.rstd_next[r]) : 1.0f, rstd_post = k.post ? *TPB_CK(&k.rstd_post[r]) : 1.0f;
+        // with FROM_X drawn here, while the row is on its way, because both halves of the work need it
+        const unsigned keep = FROM_X && k.drop.units ? keep_bits8((unsigned long long)(r * (k.width >> 3) + tid), k.drop) : 0xffu;
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         Staged<T>::sync();
         const Staged<T> st(stage_mem, (int)(r & 1), kStageArrays, nthr);
@@ -528,7 +558,25 @@ block_backward_staged_kernel(BackwardArgs<T> k) {
         if (k.next) {
             float xh[8], s = 0.0f;
             if (mine) {
-                st.read(2, xh);
+                if (FROM_X) {              // x' before it was rounded, by the forward kernel's operations
+                    st.read(3, xh);
+                    if (k.post) {
+                        weights.read(1, u);
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) xh[c] = xh[c] * rstd_post * u[c];
+                    }
+                    if (k.drop.units) drop_by8(k.drop, keep, xh);
+                    if (k.gate.p) {
+                        st.read(4, u);
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) xh[c] *= u[c];
+                    }
+                    st.read(2, u);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) xh[c] = fmaf(k.scale, xh[c], u[c]);
+                } else {
+                    st.read(2, xh);
+                }
                 st.read(1, u);
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
@@ -557,7 +605,10 @@ block_backward_staged_kernel(BackwardArgs<T> k) {
             float s = 0.0f, hat[8];
             if (mine) {
                 st.read(3, hat);
-                if (k.drop.units) drop8((unsigned long long)(r * (k.width >> 3) + tid), k.drop, t);
+                if (k.drop.units) {
+                    if (FROM_X) drop_by8(k.drop, keep, t);
+                    else drop8((unsigned long long)(r * (k.width >> 3) + tid), k.drop, t);
+                }
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     hat[c] *= rstd_post;
@@ -738,13 +789,11 @@ int backward_run(const BackwardArgs<T>& k, T* dpost, T* dnext, long long gate_gr
     const size_t smem = backward_bytes(k.width, sizeof(T), k.gate.p && !k.gate_rows);
     if (vec && k.width <= 8192 && smem <= 226 * 1024) {
         const int threads = staged_threads(k.width);
-        if (k.gate.p && !k.gate_rows) {
-            TPB_CUDA_OK(cudaFuncSetAttribute(block_backward_staged_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-            TPB_LAUNCH("block_backward_staged_kernel", (block_backward_staged_kernel<T, true>), dim3((unsigned)k.workers), threads, smem, st, k);
-        } else {
-            TPB_CUDA_OK(cudaFuncSetAttribute(block_backward_staged_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-            TPB_LAUNCH("block_backward_staged_kernel", (block_backward_staged_kernel<T, false>), dim3((unsigned)k.workers), threads, smem, st, k);
-        }
+        const bool sums = k.gate.p && !k.gate_rows;
+        const auto kernel = k.from_x ? (sums ? block_backward_staged_kernel<T, true, true> : block_backward_staged_kernel<T, false, true>)
+                                     : (sums ? block_backward_staged_kernel<T, true, false> : block_backward_staged_kernel<T, false, false>);
+        TPB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        TPB_LAUNCH("block_backward_staged_kernel", kernel, dim3((unsigned)k.workers), threads, smem, st, k);
     } else {
         TPB_BLOCK_LAUNCH(block_backward_kernel, T, p, grid, mask_bytes(p, k.width, k.drop), st, k);
     }
@@ -809,7 +858,7 @@ struct BackwardCall {
     const float *rstd_post, *rstd_next;
     void *dx, *dh, *dgate, *dpost, *dnext;
     int64_t outer, inner, width;
-    int gate_kind;
+    int gate_kind, from_x;
     double scale;
     DropSpec drop;
     Sharing share;
@@ -822,6 +871,7 @@ int backward_call(const BackwardCall& c, cudaStream_t st) {
     k.grad_y = view_of<T>(c.grad_y, c.gys);
     k.h = view_of<T>(c.h, c.hs);
     k.x_out = view_of<T>(c.x_out, c.xs);
+    k.from_x = c.from_x;
     k.gate = view_of<T>(c.gate, c.gs);
     k.post = (const T*)c.post;
     k.next = (const T*)c.next;
@@ -900,13 +950,13 @@ extern "C" size_t tpb200_block_residual_backward_workspace_bytes(int64_t outer, 
     return block_workspace(nullptr, s, width, has_post != 0, has_next != 0, sum_gate).bytes;
 }
 
-extern "C" int tpb200_block_residual_backward(const void* grad_x_out, const int64_t* grad_x_strides, const void* grad_y,
-                                              const int64_t* grad_y_strides, const void* h, const int64_t* h_strides, const void* x_out,
-                                              const int64_t* x_out_strides, const void* gate, const int64_t* gate_strides, int gate_kind,
-                                              const void* post_weight, const void* next_weight, const float* rstd_post,
-                                              const float* rstd_next, int dtype, int64_t outer, int64_t inner, int64_t width, double scale,
-                                              double p, uint64_t seed, uint64_t offset, void* grad_x, void* grad_h, void* grad_post,
-                                              void* grad_next, void* grad_gate, void* workspace, size_t workspace_bytes, void* stream) {
+static int backward_entry(const void* grad_x_out, const int64_t* grad_x_strides, const void* grad_y,
+                          const int64_t* grad_y_strides, const void* h, const int64_t* h_strides, const void* x_out,
+                          const int64_t* x_out_strides, const void* gate, const int64_t* gate_strides, int gate_kind,
+                          const void* post_weight, const void* next_weight, const float* rstd_post,
+                          const float* rstd_next, int dtype, int64_t outer, int64_t inner, int64_t width, double scale,
+                          double p, uint64_t seed, uint64_t offset, void* grad_x, void* grad_h, void* grad_post,
+                          void* grad_next, void* grad_gate, void* workspace, size_t workspace_bytes, void* stream, int from_x) {
     const int rc = check_block("block_residual_backward", dtype, outer, inner, width);
     if (rc != TPB200_OK) return rc;
     if (gate_kind < TPB200_GATE_NONE || gate_kind > TPB200_GATE_ELEMENT) return fail(TPB200_ERR_INVALID, "block_residual_backward: unknown gate kind %d", gate_kind);
@@ -940,6 +990,7 @@ extern "C" int tpb200_block_residual_backward(const void* grad_x_out, const int6
     c.dpost = c.post ? grad_post : nullptr; c.dnext = next_weight ? grad_next : nullptr;
     c.outer = outer; c.inner = inner; c.width = width;
     c.gate_kind = gated ? gate_kind : TPB200_GATE_NONE;
+    c.from_x = from_x && next_weight;
     c.scale = scale;
     const int64_t gate_rows = gate_kind == TPB200_GATE_ELEMENT ? n : gate_groups_of(gate_kind, outer);
     TPB_CHECK_RANGES(st, rows_range(c.grad_x, outer, inner, width, grad_x_strides, e), rows_range(c.grad_y, outer, inner, width, grad_y_strides, e),
@@ -952,6 +1003,29 @@ extern "C" int tpb200_block_residual_backward(const void* grad_x_out, const int6
     if (dtype == TPB200_F32) return backward_call<float>(c, st);
     if (dtype == TPB200_BF16) return backward_call<__nv_bfloat16>(c, st);
     return backward_call<__half>(c, st);
+}
+
+extern "C" int tpb200_block_residual_backward(
+    const void* grad_x_out, const int64_t* grad_x_strides, const void* grad_y, const int64_t* grad_y_strides, const void* h,
+    const int64_t* h_strides, const void* x_out, const int64_t* x_out_strides, const void* gate, const int64_t* gate_strides, int gate_kind,
+    const void* post_weight, const void* next_weight, const float* rstd_post, const float* rstd_next, int dtype, int64_t outer, int64_t inner,
+    int64_t width, double scale, double p, uint64_t seed, uint64_t offset, void* grad_x, void* grad_h, void* grad_post, void* grad_next,
+    void* grad_gate, void* workspace, size_t workspace_bytes, void* stream) {
+    return backward_entry(grad_x_out, grad_x_strides, grad_y, grad_y_strides, h, h_strides, x_out, x_out_strides, gate, gate_strides, gate_kind, post_weight,
+                          next_weight, rstd_post, rstd_next, dtype, outer, inner, width, scale, p, seed, offset, grad_x, grad_h, grad_post,
+                          grad_next, grad_gate, workspace, workspace_bytes, stream, 0);
+}
+
+extern "C" int tpb200_block_residual_backward_from_x(
+    const void* grad_x_out, const int64_t* grad_x_strides, const void* grad_y, const int64_t* grad_y_strides, const void* h,
+    const int64_t* h_strides, const void* x, const int64_t* x_strides, const void* gate, const int64_t* gate_strides, int gate_kind,
+    const void* post_weight, const void* next_weight, const float* rstd_post, const float* rstd_next, int dtype, int64_t outer, int64_t inner,
+    int64_t width, double scale, double p, uint64_t seed, uint64_t offset, void* grad_x, void* grad_h, void* grad_post, void* grad_next,
+    void* grad_gate, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!h && outer * inner * width != 0) return fail(TPB200_ERR_INVALID, "block_residual_backward: NULL pointer argument");
+    return backward_entry(grad_x_out, grad_x_strides, grad_y, grad_y_strides, h, h_strides, x, x_strides, gate, gate_strides, gate_kind, post_weight,
+                          next_weight, rstd_post, rstd_next, dtype, outer, inner, width, scale, p, seed, offset, grad_x, grad_h, grad_post,
+                          grad_next, grad_gate, workspace, workspace_bytes, stream, 1);
 }
 
 extern "C" size_t tpb200_rms_norm_backward_workspace_bytes(int64_t outer, int64_t inner, int64_t width) {

@@ -456,12 +456,16 @@ def block_residual(x, h, post_weight=None, next_weight=None, gate=None, *, scale
     return tuple(outs)
 
 
-def block_residual_backward(grad_x_out, grad_y, h, x_out, rstd_post, rstd_next, post_weight=None, next_weight=None, gate=None, *, scale=1.0,
-                            p=0.0, seed=0, offset=0, out=None):
+def block_residual_backward(grad_x_out, grad_y, h, x_out, rstd_post, rstd_next, post_weight=None, next_weight=None, gate=None, *, x=None,
+                            scale=1.0, p=0.0, seed=0, offset=0, out=None):
     """Gradients of block_residual for the gradients of x_out (None: zero) and y (with next_weight), from the
     block's output h and the forward call's x_out, rstd_post and rstd_next; weights, gate, scale, p, seed and
     offset as in that call.  Returns (grad_x, grad_h, grad_post_weight, grad_next_weight, grad_gate), None
-    where there is no such input.  `out`: these five."""
+    where there is no such input.  `out`: these five.
+
+    y was computed from x_out before it was rounded.  With `x`, the forward call's, that x_out is formed again
+    (x_out is not read then and may be None); without it the gradients go by x_out as it was rounded, and
+    grad_next_weight of a 16-bit type is off by two roundings rather than one."""
     what = "block_residual_backward"
     _check_tensor(h, what)
     size = _width(h, what)
@@ -470,12 +474,15 @@ def block_residual_backward(grad_x_out, grad_y, h, x_out, rstd_post, rstd_next, 
     kind, gs = _gate(gate, h, what)
     seed, offset = _counter(seed, offset, what)
     hs = _row_strides(h, what, "h")
-    gxs = gys = xs = None
+    gxs = gys = xs = at = None
     if grad_x_out is not None:
         gxs = _row_strides(_same(grad_x_out, h, what, "grad_x_out"), what, "grad_x_out")
     if next_weight is not None:
         gys = _row_strides(_same(grad_y, h, what, "grad_y"), what, "grad_y")
-        xs = _row_strides(_same(x_out, h, what, "x_out"), what, "x_out")
+        if x is not None:
+            at, xs = x, _row_strides(_same(x, h, what, "x"), what, "x")
+        if x is None or (x_out is not None and h.dtype == torch.float32):     # not rounded: the same bits without forming them again
+            at, xs, x = x_out, _row_strides(_same(x_out, h, what, "x_out"), what, "x_out"), None
         _rstd(rstd_next, h, what, "rstd_next")
     elif grad_y is not None:
         raise ValueError(f"{what}: grad_y without next_weight")
@@ -487,11 +494,12 @@ def block_residual_backward(grad_x_out, grad_y, h, x_out, rstd_post, rstd_next, 
         outs = _outputs(what, h, out, [same, same, row if post_weight is not None else None, row if next_weight is not None else None,
                                               (gate.shape, h.dtype) if gate is not None else None])
         if out is not None:
-            _no_overlap(what, outs, (grad_x_out, grad_y, h, x_out, rstd_post, rstd_next, post_weight, next_weight, gate))
+            _no_overlap(what, outs, (grad_x_out, grad_y, h, x_out, at, rstd_post, rstd_next, post_weight, next_weight, gate))
         nbytes = L.tpb200_block_residual_backward_workspace_bytes(*size, post_weight is not None, next_weight is not None, kind)
         ws = _scratch(nbytes, h.device)
-        _lib.check(L.tpb200_block_residual_backward(
-            _ptr(grad_x_out), gxs, _ptr(grad_y), gys, h.data_ptr(), hs, _ptr(x_out) if xs is not None else None, xs, _ptr(gate), gs, kind,
+        call = L.tpb200_block_residual_backward if x is None else L.tpb200_block_residual_backward_from_x
+        _lib.check(call(
+            _ptr(grad_x_out), gxs, _ptr(grad_y), gys, h.data_ptr(), hs, _ptr(at), xs, _ptr(gate), gs, kind,
             _ptr(post_weight), _ptr(next_weight), _ptr(rstd_post), _ptr(rstd_next), _TYPES[h.dtype], *size, scale, p, seed, offset,
             _ptr(outs[0]), _ptr(outs[1]), _ptr(outs[2]), _ptr(outs[3]), _ptr(outs[4]), _ptr(ws), nbytes, _stream(h.device)))
     return tuple(outs)

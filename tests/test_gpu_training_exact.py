@@ -1,0 +1,93 @@
+"""GPU tests of what the training operators keep of their 64-bit formulas where digits are easily lost, and of
+calls that are rarely made.  Oracles in 64 bits; every bound is derived where it stands (u = eps / 2 is one
+rounding of the output)."""
+import pytest
+import torch
+
+import training_oracle as R
+from test_gpu_training import EACH, KINDS, block_inputs
+from training_oracle import close, u
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def tpb():
+    import tensorplay_b200
+    return tensorplay_b200
+
+
+# ------------------------------------------------------------------------------------ the residual path
+
+SHAPES = pytest.mark.parametrize("shape", [(2, 3, 7), (3, 5, 64), (2, 3, 257), (3, 4, 512), (2, 30, 1000), (5, 2, 1023), (2, 9, 4096), (1, 3, 8200), (2, 2, 16384)],
+                                 ids=lambda s: "x".join(map(str, s)))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@KINDS
+@SHAPES
+def test_gradients_by_the_stream_before_it_is_rounded(cuda, tpb, dtype, kind, shape):
+    """y comes from x_out before its rounding; with x the gradients do too.  The oracle differentiates at the 64-bit
+    stream, which the kernels' float32 one is off by at most x_bound: that enters hat(x_out) as x_bound * rstd."""
+    v = block_inputs(cuda, shape, dtype, kind, 3)
+    scale, eps, how = 0.6, 1e-5, {"scale": 0.6, "p": 0.1, "seed": 11, "offset": 5}
+    x_out, y, rp, rn = tpb.block_residual(v["x"], v["h"], v["post"], v["next"], v["gate"], eps=eps, **how)
+    got = tpb.block_residual_backward(v["gx"], v["gy"], v["h"], None, rp, rn, v["post"], v["next"], v["gate"], x=v["x"], **how)
+    f = R.philox_factors(v["h"].numel(), 0.1, 11, 5, cuda).view(shape)
+    fine = R.block_forward(v["x"], v["h"], v["post"], v["next"], v["gate"], scale, eps, f)
+    back = R.block_backward(v["gx"], v["gy"], v["h"], fine["x"], rp, rn, v["post"], v["next"], v["gate"], kind, scale, f)
+    r, gy = rn.double().unsqueeze(-1), v["gy"].double()
+    hat, off = (fine["x"] * r).abs(), fine["x_bound"] * r
+    a = (gy * v["next"].double()).abs()
+    # what the stream's own error does to dL/dx, and through it to the rest
+    dt = r * (off * (a * hat).mean(-1, keepdim=True) + hat * (a * off).mean(-1, keepdim=True))
+    extra = {"next": (gy.abs() * off).flatten(0, 1).sum(0), "x": dt}
+    for name, g in zip(("x", "h", "post", "next", "gate"), got):
+        if name not in back:
+            assert g is None
+            continue
+        value, tol = (t.reshape(g.shape) for t in back[name])
+        if name in ("h", "post", "gate"):
+            # linear in dL/dx, whose magnitudes the bound multiplies by 2.4e-5 at least; dt is under 2^-19 of them
+            tol = tol * 1.1
+        else:
+            tol = tol + extra[name].reshape(g.shape)
+        close(g, value, tol + u(dtype) * value.abs() + R.TINY[dtype], f"gradient of {name}")
+
+
+@KINDS
+@SHAPES
+def test_the_stream_is_formed_again_bit_for_bit(cuda, tpb, kind, shape):
+    """In float32 x_out is not rounded further: by x or by x_out the gradients have to be the same bits."""
+    v = block_inputs(cuda, shape, torch.float32, kind, 4)
+    for post in (v["post"], None):
+        for p in (0.0, 0.3):
+            how = {"scale": -0.7, "p": p, "seed": 9, "offset": 1 << 35}
+            x_out, y, rp, rn = tpb.block_residual(v["x"], v["h"], post, v["next"], v["gate"], **how)
+            want = tpb.block_residual_backward(v["gx"], v["gy"], v["h"], x_out, rp, rn, post, v["next"], v["gate"], **how)
+            for given in (None, x_out):
+                got = tpb.block_residual_backward(v["gx"], v["gy"], v["h"], given, rp, rn, post, v["next"], v["gate"], x=v["x"], **how)
+                for a, b in zip(got, want):
+                    assert (a is None and b is None) or torch.equal(a, b)
+
+
+@EACH
+def test_x_in_place_of_x_out_as_a_view_and_without_a_next_norm(cuda, tpb, dtype):
+    v = block_inputs(cuda, (3, 9, 211), dtype, "element", 21)
+    for cut in (lambda t: t[:, 1:, 3:], lambda t: t[:, ::2, :208], lambda t: t[:, 2]):
+        w = {k: cut(t) if t.dim() == 3 else t[:cut(v["x"]).shape[-1]] for k, t in v.items()}
+        x_out, y, rp, rn = tpb.block_residual(w["x"], w["h"], w["post"], w["next"], w["gate"])
+        got = tpb.block_residual_backward(w["gx"], w["gy"], w["h"], None, rp, rn, w["post"], w["next"], w["gate"], x=w["x"])
+        c = {k: t.contiguous() for k, t in w.items()}
+        want = tpb.block_residual_backward(c["gx"], c["gy"], c["h"], None, rp, rn, c["post"], c["next"], c["gate"], x=c["x"])
+        for name, a, b in zip("xhpng", got, want):
+            # other widths of thread and worker: the same sums in another order (the oracle's bounds cover either)
+            close(a, b, 2 * u(dtype) * b.double().abs() + 1e-4 * b.double().abs().mean(), name)
+    x_out, _, rp, _ = tpb.block_residual(v["x"], v["h"], v["post"], None, v["gate"])
+    with_x = tpb.block_residual_backward(v["gx"], None, v["h"], None, rp, None, v["post"], None, v["gate"], x=v["x"])
+    plain = tpb.block_residual_backward(v["gx"], None, v["h"], x_out, rp, None, v["post"], None, v["gate"])
+    assert all((a is None and b is None) or torch.equal(a, b) for a, b in zip(with_x, plain))
+    with pytest.raises(ValueError, match="x has shape"):
+        tpb.block_residual_backward(v["gx"], v["gy"], v["h"], x_out, rp, rp, v["post"], v["next"], v["gate"], x=v["x"][:, :4])
+    with pytest.raises(TypeError, match="x_out must be a tensor"):
+        tpb.block_residual_backward(v["gx"], v["gy"], v["h"], None, rp, rp, v["post"], v["next"], v["gate"])

@@ -140,3 +140,16 @@ def test_generator_known_answers():
     f = R.philox_factors(8, 0.5, 0, 0, "cpu")
     halves = [0xE8D5, 0x6627, 0xC58D, 0xE169, 0xAC4C, 0xBC57, 0xDBD8, 0x9B00]
     assert f.tolist() == [2.0 if h >= 32768 else 0.0 for h in halves]
+
+
+def test_backward_from_x_refusals(lib):
+    """The call that takes x in place of x_out checks what the other one does, and needs h to form x_out."""
+    from tensorplay_b200 import _lib
+    S = _lib.pair(0, 8)
+
+    def back(h=PTR, x=PTR, ws=PTR, nws=1 << 30):
+        return lib.tpb200_block_residual_backward_from_x(PTR, S, PTR, S, h, S, x, S, None, S, 0, PTR, PTR, PTR, PTR, 0, 1, 4, 8, 1.0, 0.0, 0, 0,
+                                                         PTR, PTR, PTR, PTR, None, ws, nws, None)
+
+    assert back(h=None) == _lib.ERR_INVALID and back(x=None) == _lib.ERR_INVALID
+    assert back(ws=None) == _lib.ERR_WORKSPACE
