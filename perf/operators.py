@@ -215,7 +215,9 @@ def _own_block(s):
     x, y, rstd_post, rstd_next = tpb.block_residual(s["x"], s["h"], s["post"], s["next"], s["gate"], eps=EPS, **how)
     out = {"x": x, "y": y}
     if s["case"]["grad"]:
-        dx, dh, dpost, dnext, dgate = tpb.block_residual_backward(s["dx"], s["dy"], s["h"], x, rstd_post, rstd_next, s["post"], s["next"], s["gate"], **how)
+        # y went by x before its rounding: so do the gradients
+        dx, dh, dpost, dnext, dgate = tpb.block_residual_backward(s["dx"], s["dy"], s["h"], x, rstd_post, rstd_next, s["post"], s["next"], s["gate"],
+                                                                  x=s["x"], **how)
         out.update(dx=dx, dh=dh, dpost=dpost, dnext=dnext)
         if dgate is not None:
             out["dgate"] = dgate
