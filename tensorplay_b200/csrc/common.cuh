@@ -48,6 +48,12 @@ __device__ __forceinline__ T* checked(T* p, unsigned bytes, int file, int line) 
 #define TPB_CKN(p, bytes) (p)
 #endif
 
+// ------------------------------------------------------------------ cluster barrier --------
+// A CTA's shared memory may be accessed by the others of its cluster once it is known to have started.  Arriving at the
+// kernel's start and waiting just before the first access costs nothing: by then all have arrived.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
 // ------------------------------------------------------------------ loads ------------------
 // Input is read exactly once: bypass L1 allocation so the 16-byte sectors stream from L2/HBM.
 __device__ __forceinline__ float4 ld_stream4_raw(const float* p) {

@@ -546,6 +546,7 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
         if (POLICY && o) zero_part(o, Part<T>(o, in.vocab, rank, C), in.vocab, rank, C);
         return;                             // all CTAs of the cluster alike
     }
+    if (C > 1) cluster_arrive();
     const T* p = in.x + (long long)a * in.s0 + (long long)b * in.s1;
     const Part<T> part(p, in.vocab, rank, C);
     PolicyToken token{};
@@ -595,6 +596,7 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
         join_warp(s, m);
     }
     if (C > 1) {
+        cluster_wait();                     // all CTAs of the cluster have started
         if (tid < C) *cluster.map_shared_rank(&pair[rank], (unsigned)tid) = make_float2(s, m);
         cluster.sync();
         const float2 v = lane < C ? pair[lane & (kRowCluster - 1)] : make_float2(0.0f, -INFINITY);

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import training_oracle as R
-from test_gpu_training import EACH, KINDS, block_inputs
+from test_gpu_training import EACH, KINDS, block_inputs, check_policy, check_preference, check_scores, labels_of, logits_of, policy_inputs
 from training_oracle import close, u
 
 pytestmark = pytest.mark.gpu
@@ -91,3 +91,24 @@ def test_x_in_place_of_x_out_as_a_view_and_without_a_next_norm(cuda, tpb, dtype)
         tpb.block_residual_backward(v["gx"], v["gy"], v["h"], x_out, rp, rp, v["post"], v["next"], v["gate"], x=v["x"][:, :4])
     with pytest.raises(TypeError, match="x_out must be a tensor"):
         tpb.block_residual_backward(v["gx"], v["gy"], v["h"], None, rp, rp, v["post"], v["next"], v["gate"])
+
+
+# ------------------------------------------------------------------------------------ objectives on logits
+
+@EACH
+@pytest.mark.parametrize("ctas", [1, 2, 3, 5, 8])
+def test_several_ctas_per_row(cuda, tpb, dtype, ctas, monkeypatch):
+    """Rows shared by a cluster of CTAs, with the logits and the gradient on the same 16-byte boundaries and on
+    different ones (every row of an odd vocabulary starts elsewhere), and as views that shift them further."""
+    monkeypatch.setenv("TPB200_ROW_CTAS", str(ctas))
+    for vocab, cut in ((20480, slice(None)), (20011, slice(None)), (20014, slice(1, None)), (20013, slice(3, -2))):
+        x, lab, old, adv, w, ref = policy_inputs(cuda, (3, 7), vocab, dtype, vocab + ctas)
+        x = x[..., cut]
+        lab = torch.where(lab < x.shape[-1], lab, 0)
+        lp, _, _ = R.scores(x, lab)              # the cut has changed it: the older policy's by the same rule again
+        old = (lp + 0.05).float()
+        check_policy(tpb, x, lab, old, adv, w, (lp - 0.3).float())
+        check_policy(tpb, x[:, 1:], lab[:, 1:], old[:, 1:], adv[:, 1:], w[:, 1:], None, kl_coef=0.0)
+        check_scores(tpb, x[:, ::2], lab[:, ::2])
+        bounds = [(0, 4), (4, 9), (9, 20), (20, 21)]
+        check_preference(tpb, x.reshape(21, -1), lab.flatten(), (lp + 0.2).float().flatten(), bounds, torch.tensor([0, 4, 9, 20, 21], device=cuda))
