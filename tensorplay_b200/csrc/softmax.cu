@@ -233,6 +233,7 @@ softmax_long_kernel(const float* __restrict__ in, float* __restrict__ out, long 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nthr = blockDim.x;
     cg::cluster_group cluster = cg::this_cluster();
     const int c = S > 1 ? (int)cluster.block_rank() : 0;
+    if (S > 1) cluster_arrive();
     const long long r = (long long)(blockIdx.x / (unsigned)S);
     const long long a = r / k1, b = r - a * k1;
     const float* row = in + a * ks0 + b * ks1;
@@ -277,6 +278,7 @@ softmax_long_kernel(const float* __restrict__ in, float* __restrict__ out, long 
     __syncthreads();
     double sd = warp_sum(lane < nw ? sh.wsum[lane] : 0.0);
     if (S > 1) {
+        cluster_wait();  // all CTAs of the row have started
         if (tid < S) {   // this CTA's pair into every CTA of the row
             *cluster.map_shared_rank(&sh.cm[c], (unsigned)tid) = m;
             *cluster.map_shared_rank(&sh.cs[c], (unsigned)tid) = sd;

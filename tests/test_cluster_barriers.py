@@ -34,8 +34,14 @@ def test_the_check_itself():
     assert unguarded(body % ("k", 'asm volatile("barrier.cluster.wait.acquire;");')) == []
 
 
-@pytest.mark.parametrize("name", ["logprob.cu"])
+@pytest.mark.parametrize("name", ["logprob.cu", "softmax.cu", "topk_select.cuh"])
 def test_remote_shared_memory_lies_behind_a_cluster_barrier(name):
     text = open(os.path.join(CSRC, name)).read()
     assert any(REMOTE.search(k) for k in kernels(text))
     assert unguarded(text) == []
+
+
+def test_every_source_with_remote_shared_memory_is_listed():
+    files = [f for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh"))]
+    found = {f for f in files if any(REMOTE.search(k) for k in kernels(open(os.path.join(CSRC, f)).read()))}
+    assert found == {"logprob.cu", "softmax.cu", "topk_select.cuh"}
