@@ -111,8 +111,6 @@ __device__ __forceinline__ double log_sum(float s) {
     return fma((double)e, kLn2, (double)log1pf(f - 1.0f));
 }
 
-__device__ __forceinline__ double lse_of(float m, float s) { return (double)m + log_sum(s); }
-
 // ---------------------------------------------------------------- sweeps over one row --------
 // A row is a head up to the first 16-byte boundary, vectors, and a tail.
 template <class T>
@@ -605,8 +603,9 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
         join_warp(s, m);                    // the same order in every CTA
     }
     if (tid == 0) {
-        const double norm = lse_of(m, s);
-        const double logp = label < in.vocab ? (double)at_label - norm : (double)NAN;
+        // the difference from m first: m + log s would not hold log s where |m| is large (rows of a type's lowest value)
+        const double log_s = log_sum(s), norm = (double)m + log_s;
+        const double logp = label < in.vocab ? ((double)at_label - (double)m) - log_s : (double)NAN;
         if (POLICY) {
             const PolicyRow row = policy_row(terms, token, logp);
             sh.set(m, 1.0f / s, row.coef, (float)logp, label < in.vocab ? (int)label : -1);

@@ -95,6 +95,68 @@ def test_x_in_place_of_x_out_as_a_view_and_without_a_next_norm(cuda, tpb, dtype)
 
 # ------------------------------------------------------------------------------------ objectives on logits
 
+def exact_rows(x, labels):
+    """(logp, p of every entry, 1 - p of the label) in 64 bits, from differences to the row's maximum and with the label
+    left out of the sum: neither a large common value nor a p near 1 costs digits."""
+    d = x.double() - x.double().amax(-1, keepdim=True)
+    hit = torch.nn.functional.one_hot(labels, x.shape[-1]).bool()
+    e = d.exp()
+    others = torch.where(hit, 0.0, e).sum(-1)
+    own = d.gather(-1, labels.unsqueeze(-1)).squeeze(-1)
+    total = others + own.exp()
+    logp = torch.where(own > others.log(), -torch.log1p(others / own.exp()), own - total.log())
+    return logp, e / total.unsqueeze(-1), others / total, hit
+
+
+def grad_rows(x, labels, coef):
+    _, p, rest, hit = exact_rows(x, labels)
+    return torch.where(hit, rest.unsqueeze(-1), -p) * coef.double().unsqueeze(-1)
+
+
+def far_rows(cuda, dtype, vocab):
+    """Rows around values that a float64 sum with log V does not hold beside it, or only in part."""
+    top = torch.finfo(dtype).max
+    fill = [-top, top / 2, -top / 3, 4e4, -3e3] + ([1e16, -2.0 ** 60, 3e7, 2.0 ** 28] if dtype != torch.float16 else [])
+    x = torch.stack([torch.full((vocab,), f, device=cuda, dtype=torch.float64) for f in fill])
+    x[:, 1::3] -= x[:, 1::3].abs() * (4 * u(dtype))          # a third of the entries a few steps lower
+    x = x.to(dtype)
+    # all entries alike, and a label that is one of the lower ones
+    x = torch.cat([x, torch.full((2, vocab), -top, device=cuda, dtype=dtype)])
+    labels = torch.arange(x.shape[0], device=cuda) % 4
+    return x, labels
+
+
+@EACH
+@pytest.mark.parametrize("vocab", [5, 777, 20011])
+def test_rows_around_large_values(cuda, tpb, dtype, vocab):
+    """A row that a mask has filled with the type's lowest value is a uniform row: logp = -log V and a gradient.
+    Bounds: P of the sums, as in the oracle's file; no term in |lse|."""
+    x, lab = far_rows(cuda, dtype, vocab)
+    n = x.shape[0]
+    logp, p, rest, hit = exact_rows(x, lab)
+    assert bool((logp[-2:] + torch.tensor(float(vocab)).log().to(cuda) < 1e-6).all()) and bool(logp[-2:].ne(0).all())
+    tol = R.P + u(torch.float32) * logp.abs()
+    close(tpb.token_logprobs(x, lab)[0], logp, tol, "logp of token_logprobs")
+    one = torch.ones(n, device=cuda)
+    old = logp.clamp_min(-50).float()                        # a ratio near 1, or 0 where the label is far below
+    loss, grad, got, ratio, kl = tpb.policy_loss(x, lab, old, one, one / n)
+    close(got, logp, tol, "logp of policy_loss")
+    r = (logp - old.double()).exp()
+    close(ratio, r, r * (R.P + 2.0 ** -21), "ratio")
+    g = grad_rows(x, lab, -r / n)
+    close(grad, g, g.abs() * (2 * R.P + 2.0 ** -20 + u(dtype)) + R.TINY[dtype], "gradient of policy_loss")
+    n -= n % 2
+    _, grad, rewards, got = tpb.preference_loss(x[:n], lab[:n], old[:n], torch.arange(n + 1, device=cuda), beta=0.3)
+    close(got, logp[:n], tol[:n], "logp of preference_loss")
+    s = torch.where(logp[:n] < -1e30, 0.0, 0.3 * (logp[:n] - old[:n].double()))
+    m = (s[0::2] - s[1::2])
+    near = (logp[:n].view(-1, 2) > -1e30).all(1)             # pairs whose margin is a number that float32 holds
+    slope = -0.3 * torch.sigmoid(-m) / (n // 2)
+    g = grad_rows(x[:n], lab[:n], torch.stack([slope, -slope], 1).flatten())
+    keep = near.repeat_interleave(2)
+    close(grad[keep], g[keep], (g.abs() * (2 * R.P + 0.3 * 2 * R.P + 2.0 ** -20 + u(dtype)) + R.TINY[dtype])[keep], "gradient of preference_loss")
+
+
 @EACH
 @pytest.mark.parametrize("ctas", [1, 2, 3, 5, 8])
 def test_several_ctas_per_row(cuda, tpb, dtype, ctas, monkeypatch):
