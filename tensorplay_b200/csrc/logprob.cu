@@ -3,18 +3,19 @@
 // tpb200_policy_loss and tpb200_preference_loss.
 //
 // Mathematics.  For a row x of V logits and its token y, in base 2 with c = log2(e):
-//     m = max_j x_j,   s = sum_j 2^(c (x_j - m)),   lse = m + log2(s) / c,   logp = x_y - lse
-//     d logp / d x_j = [j = y] - p_j,   p_j = 2^(c (x_j - m)) / s
+//     m = max_j x_j,   s = sum over j != y of 2^(c (x_j - m)),   g = (x_y - m) - log2(s) / c
+//     logp = -log(1 + e^-g),   1 - p_y = 1 / (1 + e^g),   p_j = (1 - p_y) 2^(c (x_j - m)) / s,   d logp / d x_j = [j = y] - p_j
 // so every loss that depends on x through logp alone has the gradient coef * ([j = y] - p_j) with one
-// number `coef` per row.  c is the float32 nearest to log2(e) and is divided out again in 64 bits.  m may be any
+// number `coef` per row.  The token's own term stays out of the sum: g, the log of its odds against all others,
+// holds the digits of 1 - p_y however near p_y is to 1 (most tokens of a trained model), where a sum of all would hold
+// p_y alone, and the rows of the gradient add up to zero.  c is the float32 nearest to log2(e) and is divided out again in 64 bits.  m may be any
 // reference near the maximum.  The hot loops take the exponent as one fused multiply-add, c x - M with
 // M = fl(c m): the product is exact there, and M's own rounding, c m - M, is one factor per row (or thread) that
 // is taken out once.  Where |m| >= 2^28 that factor leaves the range of float32 (rows of a type's lowest
 // value are such rows); there x - m is formed first.
 //   * s is kept in float32, a few hundred terms per thread at most, and joined by trees;
-//   * the per-row scalars (log s, logp, differences of log-probabilities) are formed in float64 from an
-//     exponent and a mantissa, the gradient at the token itself is coef * -expm1(logp), which keeps its
-//     digits where p_y is near 1.
+//   * the per-row scalars (log s, g, logp, differences of log-probabilities) are formed in float64 from an
+//     exponent and a mantissa; the gradient at the token itself is coef * (1 - p_y).
 // A token with a negative label or a weight of zero takes no part: its row is not read, its outputs and
 // its gradient are zero.  A label of V or more gives NaN, never an access outside the row.
 #define TPB_FILE_ID 7
@@ -111,6 +112,41 @@ __device__ __forceinline__ double log_sum(float s) {
     return fma((double)e, kLn2, (double)log1pf(f - 1.0f));
 }
 
+// What a row's sum over the other entries says of its token.  e^-|g| is rounded to float32, 2^-23 of itself, logarithms are
+// float32 below 0.7: logp is within 2^-22 of itself, or 1e-7 where it is large.
+struct Score {
+    double logp, lse;
+    float gap, e;                // g, NaN for a label beyond the vocabulary, and e^-|g|
+    // 1 - p_y
+    __device__ __forceinline__ float rest() const { return gap != gap ? NAN : __fdividef(gap >= 0.0f ? e : 1.0f, 1.0f + e); }
+};
+// x_y, and (reference, sum) of the others; `known`: the label lies in the vocabulary
+__device__ __forceinline__ Score score_of(bool known, float own, float m, float s) {
+    Score o;
+    const double log_s = log_sum(s);
+    // the difference from m first: m + log s would not hold log s where |m| is large (rows of a type's lowest value)
+    const double gap = ((double)own - (double)m) - log_s;
+    o.gap = known && own < INFINITY ? (float)gap : NAN;
+    const float low = (float)(gap - (double)o.gap);           // NaN where gap is infinite: e is 0 then
+    o.e = expf(-fabsf(o.gap));
+    if (o.e > 0.0f) o.e = fmaf(o.e, o.gap < 0.0f ? low : -low, o.e);
+    const float l = log1pf(o.e);
+    if (o.gap >= 0.0f) {
+        o.logp = (double)(0.0f - l);
+        o.lse = (double)(own + l);
+    } else {                                                  // NaN too
+        o.logp = (o.gap != o.gap ? (double)NAN : gap) - (double)l;
+        o.lse = known ? ((double)m + log_s) + (double)l : (double)m + log_s;
+    }
+    return o;
+}
+// `unit` such that p_j = unit * 2^(c (x_j - reference)) for the others, and the reference.  Where there are none (a vocabulary
+// of one, or all of them -inf) they have no share.
+__device__ __forceinline__ float2 unit_of(const Score& y, float own, float m, float s) {
+    const float rest = y.rest();
+    return s == 0.0f ? make_float2(own, rest) : make_float2(m, __fdividef(rest, s));
+}
+
 // ---------------------------------------------------------------- sweeps over one row --------
 // A row is a head up to the first 16-byte boundary, vectors, and a tail.
 template <class T>
@@ -134,14 +170,14 @@ __device__ __forceinline__ float residue(float m, float M) { return fmaf(m, kLog
 struct RowGrad {
     float m, M, k, at_label;
     int label, far;
-    // from the reference, the sum of 2^(c (x - m)) (its reciprocal), the coefficient and logp
-    __device__ __forceinline__ void set(float reference, float inv_s, float coef, float logp, int at) {
+    // from the reference, `unit` and 1 - p_y of the row's score, and the coefficient
+    __device__ __forceinline__ void set(float reference, float unit, float rest, float coef, int at) {
         m = reference;
         far = !(fabsf(m) < kFar);
         M = far ? 0.0f : m * kLog2e;
-        k = -coef * inv_s;
+        k = -coef * unit;
         if (!far) k *= ex2(-residue(m, M));
-        at_label = coef * -expm1f(logp);
+        at_label = coef * rest;
         label = at;
     }
     __device__ __forceinline__ float value(float x) const { return k * ex2(far ? (x - m) * kLog2e : fmaf(x, kLog2e, -M)); }
@@ -327,6 +363,19 @@ template <> struct VecMax<__half> {
     __device__ __forceinline__ float get() const { return fmaxf(__low2float(m), __high2float(m)); }
 };
 
+// -inf in place of element e of VECS vectors
+template <class T, int VECS>
+__device__ __forceinline__ void leave_out(uint4 (&raw)[VECS], int e) {
+    constexpr int per = 4 / (int)sizeof(T);     // elements of a word
+#pragma unroll
+    for (int u = 0; u < VECS; ++u)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            uint32_t& x = w == 0 ? raw[u].x : w == 1 ? raw[u].y : w == 2 ? raw[u].z : raw[u].w;
+            if (e / per == u * 4 + w) x = per == 1 ? Elem<T>::kNegInf : __byte_perm(x, Elem<T>::kNegInf, e & 1 ? 0x5410 : 0x3254);
+        }
+}
+
 // Running sum of 2^(c x - M) of one thread over a row, two vectors at a time, against a reference that is fixed
 // after the first of them: no maximum and no rescaling per element.  A step whose sum is not below 2^60 --
 // values far above the reference, infinities, NaN, far rows (their M is NaN) -- is done again the careful
@@ -475,7 +524,7 @@ __global__ void __launch_bounds__(32) pair_sum_kernel(PairSum sum) { sum.run(); 
 
 struct ScoreOut {
     float *logp, *lse;   // all but logp may be NULL
-    float2* keep;        // (reference, 1 / s)
+    float2* keep;        // (reference, unit)
     double* exact;       // logp before it is rounded
     float* coef;         // set to zero: rows of no sequence keep that
 };
@@ -515,6 +564,7 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
     __shared__ float red_s[kRowThreads / 32], red_m[kRowThreads / 32];
     __shared__ float2 pair[kRowCluster];     // (sum, reference) of every CTA of the cluster
     __shared__ RowGrad sh;
+    __shared__ int skipped[kRowThreads / 32];   // the place of the token's entry in its vector, for every warp
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nthr = blockDim.x;
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = C > 1 ? (int)cluster.block_rank() : 0;
@@ -556,7 +606,11 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
     const int edge = part.edge(tid, in.vocab, rank, C);
     const float edge_x = edge >= 0 ? Elem<T>::get(*TPB_CK(&p[edge])) : -INFINITY;
 
-    // ---- the sum
+    // ---- the sum of all but the token's own term
+    const int at = label < in.vocab ? (int)label : -1;
+    const int skip = at >= part.head && at < in.vocab - part.tail ? (at - part.head) / N - part.first : -1;   // the vector with the token's entry
+    if (lane == 0) skipped[warp] = (at - part.head) & (N - 1);
+    __syncwarp();
     const T* q = p + part.head + (size_t)part.first * N;
     FixedSum<T> sum;
     sum.init();
@@ -565,14 +619,17 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
         const unsigned long long policy = POLICY && o ? l2_last() : l2_first();
         int i = tid;
         for (; i + nthr < part.n; i += 2 * nthr) {
-            const uint4 raw[2] = {ld_policy16(q + (size_t)i * N, policy), ld_policy16(q + (size_t)(i + nthr) * N, policy)};
+            uint4 raw[2] = {ld_policy16(q + (size_t)i * N, policy), ld_policy16(q + (size_t)(i + nthr) * N, policy)};
+            const int d = skip - i;
+            if (d == 0 || d == nthr) leave_out<T>(raw, (d == 0 ? 0 : N) + skipped[warp]);
             sum.add(raw, i == tid);
         }
         if (i < part.n) {
-            const uint4 raw[1] = {ld_policy16(q + (size_t)i * N, policy)};
+            uint4 raw[1] = {ld_policy16(q + (size_t)i * N, policy)};
+            if (i == skip) leave_out<T>(raw, skipped[warp]);
             sum.add(raw, i == tid);
         }
-        if (edge >= 0) {                    // as a vector with one element
+        if (edge >= 0 && edge != at) {      // as a vector with one element
             float v[N];
 #pragma unroll
             for (int e = 0; e < N; ++e) v[e] = e == 0 ? edge_x : -INFINITY;
@@ -603,21 +660,20 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
         join_warp(s, m);                    // the same order in every CTA
     }
     if (tid == 0) {
-        // the difference from m first: m + log s would not hold log s where |m| is large (rows of a type's lowest value)
-        const double log_s = log_sum(s), norm = (double)m + log_s;
-        const double logp = label < in.vocab ? ((double)at_label - (double)m) - log_s : (double)NAN;
+        const Score y = score_of(at >= 0, at_label, m, s);
         if (POLICY) {
-            const PolicyRow row = policy_row(terms, token, logp);
-            sh.set(m, 1.0f / s, row.coef, (float)logp, label < in.vocab ? (int)label : -1);
+            const PolicyRow row = policy_row(terms, token, y.logp);
+            const float2 k = unit_of(y, at_label, m, s);
+            sh.set(k.x, k.y, y.rest(), row.coef, at);
             if (rank == 0) {
-                store_policy(out, r, logp, row);
+                store_policy(out, r, y.logp, row);
                 if (loss) *TPB_CK(loss) = (float)row.part;
             }
         } else if (rank == 0) {
-            *TPB_CK(&score.logp[r]) = (float)logp;
-            if (score.lse) *TPB_CK(&score.lse[r]) = (float)norm;
-            if (score.keep) *TPB_CK(&score.keep[r]) = make_float2(m, 1.0f / s);
-            if (score.exact) *TPB_CK(&score.exact[r]) = logp;
+            *TPB_CK(&score.logp[r]) = (float)y.logp;
+            if (score.lse) *TPB_CK(&score.lse[r]) = (float)y.lse;
+            if (score.keep) *TPB_CK(&score.keep[r]) = unit_of(y, at_label, m, s);
+            if (score.exact) *TPB_CK(&score.exact[r]) = y.logp;
             if (score.coef) *TPB_CK(&score.coef[r]) = 0.0f;
         }
     }
@@ -655,10 +711,10 @@ score_grad_kernel(Logits<T> in, PerToken<long long> labels, PerToken<float> grad
     const int at = y < in.vocab ? (int)y : -1;
     if (keep) {
         const float2 k = *TPB_CK(&keep[r]);
-        g.set(k.x, k.y, coef, *TPB_CK(&logp[r]), at);
+        g.set(k.x, k.y, -expm1f(*TPB_CK(&logp[r])), coef, at);
     } else {
         const float n = *TPB_CK(&lse[r]);      // p = 2^(c (x - lse))
-        g.set(n, 1.0f, coef, y < in.vocab ? (float)((double)Elem<T>::get(*TPB_CK(&p[y])) - (double)n) : NAN, at);
+        g.set(n, 1.0f, -expm1f(y < in.vocab ? (float)((double)Elem<T>::get(*TPB_CK(&p[y])) - (double)n) : NAN), coef, at);
     }
     if (y >= in.vocab) g.k = NAN;
     grad_part(p, o, part, g, edge, edge_x);
@@ -889,7 +945,7 @@ extern "C" int tpb200_policy_loss(const void* logits, int dtype, int64_t outer, 
     return TPB200_OK;
 }
 
-// workspace of the preference loss: logp in 64 bits, (reference, 1 / s) and the coefficient of every row, the loss of every pair
+// workspace of the preference loss: logp in 64 bits, (reference, unit) and the coefficient of every row, the loss of every pair
 extern "C" size_t tpb200_preference_loss_workspace_bytes(int64_t outer, int64_t inner, int64_t pairs) {
     if (outer < 0 || inner < 0 || pairs < 0) return 0;
     return (size_t)(outer * inner) * (sizeof(double) + sizeof(float2) + sizeof(float)) + (size_t)pairs * sizeof(double);

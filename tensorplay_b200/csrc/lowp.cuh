@@ -13,6 +13,7 @@ template <class T> struct Elem;
 
 template <> struct Elem<float> {
     static constexpr int N = 4;   // elements of a 16-byte vector
+    static constexpr uint32_t kNegInf = 0xff800000u;
     static __device__ __forceinline__ float get(float v) { return v; }
     static __device__ __forceinline__ float put(float v) { return v; }
     static __device__ __forceinline__ void unpack(const uint4& v, float* f) {
@@ -25,6 +26,7 @@ template <> struct Elem<float> {
 
 template <> struct Elem<__nv_bfloat16> {
     static constexpr int N = 8;
+    static constexpr uint32_t kNegInf = 0xff80u;
     static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
     static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
     // a bfloat16 is the upper half of a float32
@@ -46,6 +48,7 @@ template <> struct Elem<__nv_bfloat16> {
 
 template <> struct Elem<__half> {
     static constexpr int N = 8;
+    static constexpr uint32_t kNegInf = 0xfc00u;
     static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
     static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
     static __device__ __forceinline__ void two(uint32_t w, float* f) {

@@ -174,3 +174,52 @@ def test_several_ctas_per_row(cuda, tpb, dtype, ctas, monkeypatch):
         check_scores(tpb, x[:, ::2], lab[:, ::2])
         bounds = [(0, 4), (4, 9), (9, 20), (20, 21)]
         check_preference(tpb, x.reshape(21, -1), lab.flatten(), (lp + 0.2).float().flatten(), bounds, torch.tensor([0, 4, 9, 20, 21], device=cuda))
+
+
+def confident(cuda, dtype, vocab, seed):
+    """Rows whose token has nearly all of the probability, at the places where a row begins, ends and is split."""
+    places = sorted({0, 1, vocab // 3, vocab // 2 + 1, vocab - 2, vocab - 1} & set(range(vocab)))
+    heights = [10.0, 14.0, 17.0, 20.0, 28.0, 30.0, 45.0, 80.0]
+    lab = torch.tensor([i for i in places for _ in heights], device=cuda)
+    x = logits_of(cuda, (lab.numel(), vocab), dtype, seed, spread=2.0)
+    up = torch.tensor(heights, device=cuda).repeat(len(places))
+    return x.scatter(1, lab.unsqueeze(1), up.to(dtype).unsqueeze(1)), lab
+
+
+@EACH
+@pytest.mark.parametrize("vocab,shift", [(2, 0), (9, 0), (77, 1), (1000, 0), (32000, 0), (50021, 0), (50048, 3), (151936, 0)])
+def test_tokens_with_a_probability_near_one(cuda, tpb, dtype, vocab, shift):
+    """logp = -(1 - p) and the token's gradient are held to P of themselves, from 1 - p = 0.9 down to e^-80; the sum of the
+    others is off by at most P of itself, e^-|g|, its logarithm and the products by 2^-20 of themselves.  No logp is
+    positive, and a row of the gradient adds up to zero."""
+    x, lab = confident(cuda, dtype, vocab + shift, 7 + vocab)
+    x, lab = x[:, shift:], (lab - shift).clamp_min(0)
+    logp, p, rest, hit = exact_rows(x, lab)
+    rel = R.P + 2.0 ** -20
+    got, lse = tpb.token_logprobs(x, lab)
+    assert bool((got <= 0).all())
+    close(got, logp, logp.abs() * rel + R.TINY[torch.float32], "logp of token_logprobs")
+    close(lse, x.double().logsumexp(1), R.P + u(torch.float32) * lse.double().abs(), "lse")
+    n = lab.numel()
+    one = torch.ones(n, device=cuda)
+    old = (logp + 0.1).float()
+    loss, grad, got, ratio, _ = tpb.policy_loss(x, lab, old, one, one, grad_scale=64.0)
+    close(got, logp, logp.abs() * rel + R.TINY[torch.float32], "logp of policy_loss")
+    r = (logp - old.double()).exp()
+    g = grad_rows(x, lab, -64.0 * r)
+    # every entry: its own exponential (P) and the sum's
+    tol = g.abs() * (2 * R.P + 2.0 ** -19 + u(dtype)) + R.TINY[dtype]
+    close(grad, g, tol, "gradient of policy_loss")
+    if dtype == torch.float32:
+        # V terms of up to 2^-23 of themselves, each with its own exponential's error of 2^-22 and P / 8 of the sweep
+        total, size = grad.double().sum(1).abs(), g.abs().sum(1)
+        assert bool((total <= size * (R.P + 2.0 ** -22) + R.TINY[dtype] * vocab).all())
+    n -= n % 2
+    ref = (logp + 0.2).float()
+    offsets = torch.arange(n + 1, device=cuda)
+    _, grad, rewards, got = tpb.preference_loss(x[:n], lab[:n], ref[:n], offsets, beta=0.5, grad_scale=1024.0)
+    close(got, logp[:n], logp[:n].abs() * rel + R.TINY[torch.float32], "logp of preference_loss")
+    m = 0.5 * (logp - ref.double())[:n]
+    slope = -1024.0 * 0.5 * torch.sigmoid(-(m[0::2] - m[1::2])) / (n // 2)
+    g = grad_rows(x[:n], lab[:n], torch.stack([slope, -slope], 1).flatten())
+    close(grad, g, g.abs() * (3 * R.P + 2.0 ** -19 + u(dtype)) + R.TINY[dtype], "gradient of preference_loss")
