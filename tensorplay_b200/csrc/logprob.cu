@@ -8,11 +8,13 @@
 // so every loss that depends on x through logp alone has the gradient coef * ([j = y] - p_j) with one
 // number `coef` per row.  The token's own term stays out of the sum: g, the log of its odds against all others,
 // holds the digits of 1 - p_y however near p_y is to 1 (most tokens of a trained model), where a sum of all would hold
-// p_y alone, and the rows of the gradient add up to zero.  c is the float32 nearest to log2(e) and is divided out again in 64 bits.  m may be any
-// reference near the maximum.  The hot loops take the exponent as one fused multiply-add, c x - M with
-// M = fl(c m): the product is exact there, and M's own rounding, c m - M, is one factor per row (or thread) that
-// is taken out once.  Where |m| >= 2^28 that factor leaves the range of float32 (rows of a type's lowest
-// value are such rows); there x - m is formed first.
+// p_y alone, and the rows of the gradient add up to zero.  m may be any reference near the maximum.
+//   * Sums go by an integer E near c m, c x - E, so that sums of threads and CTAs are joined by exact powers of two, and by
+//     c to 1e-10 of itself (FixedSum): a base that is off by d shifts every log s to the same side, by d times the mean
+//     distance of the logits, and a reward adds that up over its sequence.  (With c a float32 rewards of [3001,151936]
+//     were 1.2e-6 of themselves off.)  The gradient, whose entries stand by themselves, takes one multiply-add
+//     with the float32 c.
+//   * Where |m| >= 2^12 (rows of a type's lowest value are such rows) x - m is formed first.
 //   * s is kept in float32, a few hundred terms per thread at most, and joined by trees;
 //   * the per-row scalars (log s, g, logp, differences of log-probabilities) are formed in float64 from an
 //     exponent and a mantissa; the gradient at the token itself is coef * (1 - p_y).
@@ -31,6 +33,16 @@ namespace tpb {
 namespace cg = cooperative_groups;
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLn2 = 0.6931471805599453;
+// log2(e) = kStep + kRest to 1.2e-10 of itself; kStep has five bits, so that kStep x - E is exact for 16-bit types
+constexpr float kStep = 1.4375f, kRest = 1.4426950408889634 - 1.4375;
+// e^v = 2^(kLog2e v) times e^(kLow c v): what the float32 c leaves out
+constexpr float kLow = (1.4426950408889634 - (double)kLog2e) / 1.4426950408889634 * kLn2;
+// ex2.approx is low by this on average over an octave of negative arguments (2^22 of them measured, each off by at most
+// 1.5e-7); a sum of many terms is low by as much, always to the same side
+constexpr double kExLow = 5.0e-8;
+constexpr float kFar = 4096.0f;          // |reference| from which x - m is formed first
+constexpr float kAbove = 6.0f;           // octaves of E above the reference, so that no argument of ex2 is above 1
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -63,7 +75,18 @@ __device__ __forceinline__ unsigned long long fma2(unsigned long long x, unsigne
     return r;
 }
 
-// v[i] := 2^(c v[i] - M), or 2^(c (v[i] - m)), for an even number of values
+// v[i] := 2^(c v[i] - E), 2^(kLog2e v[i] - M), or 2^(c (v[i] - m)), for an even number of values
+template <int N>
+__device__ __forceinline__ void exps_fine(float (&v)[N], float E) {
+    const unsigned long long neg = bits_of(-E, -E), step = bits_of(kStep, kStep), rest = bits_of(kRest, kRest);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const unsigned long long x = bits_of(v[i], v[i + 1]);
+        const Two t = two_of(fma2(x, rest, fma2(x, step, neg)));
+        v[i] = ex2(t.a);
+        v[i + 1] = ex2(t.b);
+    }
+}
 template <int N>
 __device__ __forceinline__ void exps_fma(float (&v)[N], float M) {
     const unsigned long long neg = bits_of(-M, -M), c = bits_of(kLog2e, kLog2e);
@@ -100,15 +123,27 @@ struct Logits {
     int vocab;
 };
 
-// log(s) of a row's sum (float32 or joined in float64, rounded to float32 here: 2^-25 of it): the exponent
-// and the logarithm of a mantissa in [1/sqrt 2, sqrt 2), so that the float32 part is below 0.35.  In base
-// 2^(1/c) the logarithm is that of log2(s) / c.  No float64 division on the way: one costs a row some 0.5 us.
+// What the sums of a reference m are relative to: 2^E, an integer E near c m, or, for a far one, e^m.
+__device__ __forceinline__ bool near(float m) { return fabsf(m) < kFar; }
+__device__ __forceinline__ float base_of(float m) { return rintf(m * kLog2e) + kAbove; }
+// a sum that is relative to `own` as one relative to m >= own
+__device__ __forceinline__ float rebase(float own, float m) {
+    if (own == m) return 1.0f;
+    if (near(own) && near(m)) {
+        const float d = base_of(own) - base_of(m);
+        return d > -126.0f ? __int_as_float(((int)d + 127) << 23) : 0.0f;
+    }
+    const float r = near(own) ? fmaf(own, -kLog2e, base_of(own)) : 0.0f, t = near(m) ? fmaf(m, -kLog2e, base_of(m)) : 0.0f;
+    return ex2((own - m) * kLog2e + (r - t));      // own = -inf: 0
+}
+
+// log(s) of a row's sum: the exponent and the logarithm of a mantissa in [1/sqrt 2, sqrt 2), so that the float32 part is
+// below 0.35.  No float64 division on the way: one costs a row some 0.5 us.
 __device__ __forceinline__ double log_sum(float s) {
     if (!(s >= 1.17549435e-38f && s < INFINITY)) return (double)logf(s);   // 0, NaN, inf
     int e = (int)(__float_as_uint(s) >> 23) - 127;
     float f = __uint_as_float((__float_as_uint(s) & 0x007fffffu) | 0x3f800000u);
     if (f > 1.41421356f) { f *= 0.5f; ++e; }
-    constexpr double kLn2 = 1.0 / (double)kLog2e;       // of the c that the sweeps use
     return fma((double)e, kLn2, (double)log1pf(f - 1.0f));
 }
 
@@ -123,9 +158,9 @@ struct Score {
 // x_y, and (reference, sum) of the others; `known`: the label lies in the vocabulary
 __device__ __forceinline__ Score score_of(bool known, float own, float m, float s) {
     Score o;
-    const double log_s = log_sum(s);
-    // the difference from m first: m + log s would not hold log s where |m| is large (rows of a type's lowest value)
-    const double gap = ((double)own - (double)m) - log_s;
+    const double log_s = log_sum(s) + kExLow, base = near(m) ? (double)base_of(m) * kLn2 : (double)m;
+    // the difference from the base first: base + log s would not hold log s where |m| is large (rows of a type's lowest value)
+    const double gap = ((double)own - base) - log_s;
     o.gap = known && own < INFINITY ? (float)gap : NAN;
     const float low = (float)(gap - (double)o.gap);           // NaN where gap is infinite: e is 0 then
     o.e = expf(-fabsf(o.gap));
@@ -136,11 +171,11 @@ __device__ __forceinline__ Score score_of(bool known, float own, float m, float 
         o.lse = (double)(own + l);
     } else {                                                  // NaN too
         o.logp = (o.gap != o.gap ? (double)NAN : gap) - (double)l;
-        o.lse = known ? ((double)m + log_s) + (double)l : (double)m + log_s;
+        o.lse = known ? (base + log_s) + (double)l : base + log_s;
     }
     return o;
 }
-// `unit` such that p_j = unit * 2^(c (x_j - reference)) for the others, and the reference.  Where there are none (a vocabulary
+// The reference, and `unit` such that p_j = unit * 2^(c x_j - E) for the others (far: unit * e^(x_j - m)).  Where there are none (a vocabulary
 // of one, or all of them -inf) they have no share.
 __device__ __forceinline__ float2 unit_of(const Score& y, float own, float m, float s) {
     const float rest = y.rest();
@@ -161,22 +196,18 @@ struct Span {
     }
 };
 
-constexpr float kFar = 268435456.0f;     // 2^28
-// c m - M for M = fl(c m): the rounding of M, exactly
-__device__ __forceinline__ float residue(float m, float M) { return fmaf(m, kLog2e, -M); }
-
-// What the gradient of one row needs: g_j = k * 2^(c x_j - M), or k * 2^(c (x_j - m)) for a far row, and
-// `at_label` in the token's place.
+// What the gradient of one row needs: g_j = k * 2^(kLog2e x_j - M), M = E, or k * 2^(c (x_j - m)) for a far row, and
+// `at_label` in the token's place.  k holds what the float32 c leaves out at x = m; 1.3e-8 of x_j - m remain.
 struct RowGrad {
     float m, M, k, at_label;
     int label, far;
     // from the reference, `unit` and 1 - p_y of the row's score, and the coefficient
     __device__ __forceinline__ void set(float reference, float unit, float rest, float coef, int at) {
         m = reference;
-        far = !(fabsf(m) < kFar);
-        M = far ? 0.0f : m * kLog2e;
+        far = !near(m);
+        M = far ? 0.0f : base_of(m);
         k = -coef * unit;
-        if (!far) k *= ex2(-residue(m, M));
+        if (!far) k = fmaf(k, kLow * M, k);
         at_label = coef * rest;
         label = at;
     }
@@ -274,10 +305,17 @@ __device__ __forceinline__ float kl_term(float d) {
     return expm1f(d) - d;
 }
 
-// A token's inputs, fetched before the row is swept.
+// A token's inputs, fetched before the row is swept, asynchronously into shared memory: the sweep has no register to
+// spare for them ([4096,151936] bf16: 545 us with them in registers, 534 so).
 struct PolicyToken { float old_logp, advantage, weight, ref; };
-__device__ __forceinline__ PolicyToken policy_token(const PolicyTerms& t, long long a, long long b, float w) {
-    return PolicyToken{t.old_logp.at(a, b), t.advantage.at(a, b), w, t.ref.p ? t.ref.at(a, b) : 0.0f};
+__device__ __forceinline__ void copy_async4(float* dst, const float* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(TPB_CK(src)) : "memory");
+}
+__device__ __forceinline__ void fetch_token(const PolicyTerms& t, long long a, long long b, float w, PolicyToken* k) {
+    copy_async4(&k->old_logp, t.old_logp.p + a * t.old_logp.s0 + b * t.old_logp.s1);
+    copy_async4(&k->advantage, t.advantage.p + a * t.advantage.s0 + b * t.advantage.s1);
+    k->weight = w;
+    if (t.ref.p) copy_async4(&k->ref, t.ref.p + a * t.ref.s0 + b * t.ref.s1);
 }
 
 // The row's outputs and its coefficient d loss / d logp:
@@ -363,6 +401,13 @@ template <> struct VecMax<__half> {
     __device__ __forceinline__ float get() const { return fmaxf(__low2float(m), __high2float(m)); }
 };
 
+__device__ __forceinline__ unsigned lanes_below(int n) { return n >= 32 ? kFull : n <= 0 ? 0u : (1u << n) - 1u; }
+__device__ __forceinline__ float lanes_max(float v, unsigned mask) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "r"(mask));
+    return r;
+}
+
 // -inf in place of element e of VECS vectors
 template <class T, int VECS>
 __device__ __forceinline__ void leave_out(uint4 (&raw)[VECS], int e) {
@@ -376,58 +421,60 @@ __device__ __forceinline__ void leave_out(uint4 (&raw)[VECS], int e) {
         }
 }
 
-// Running sum of 2^(c x - M) of one thread over a row, two vectors at a time, against a reference that is fixed
-// after the first of them: no maximum and no rescaling per element.  A step whose sum is not below 2^60 --
-// values far above the reference, infinities, NaN, far rows (their M is NaN) -- is done again the careful
-// way, which raises the reference.  (A running maximum took 25 instructions per element in all, this 14.)
+// Running sum of 2^(c x - E) of one thread over a row, two vectors at a time, against a reference that is fixed
+// after the first step, the maximum of what the warp has met there: no maximum and no rescaling per element.  A step
+// whose sum is not below 2 -- values well above the reference, infinities, NaN, far rows (their E is NaN) -- is done
+// again the careful way, which raises the reference.  (A running maximum took 25 instructions per element in all, this
+// 14.)  The exponent is kRest x + (kStep x - E): two roundings, of 2^-22 at most for float32 below 8 and |x| below 1500, the
+// first of them none for a 16-bit type.
 template <class T>
 struct FixedSum {
     static constexpr int N = Elem<T>::N;
-    float ref, M, s;      // ref = -inf: nothing but -inf and NaN so far; M = NaN then, and for a far reference
-    __device__ __forceinline__ void init() { ref = -INFINITY; M = NAN; s = 0.0f; }
-    // s relative to 2^(c ref) rather than 2^M, and back
-    __device__ __forceinline__ float out(float v) const { return M != M ? v : v * ex2(-residue(ref, M)); }
-    __device__ __forceinline__ float in(float v) const { return M != M ? v : v * ex2(residue(ref, M)); }
+    float ref, E, s;      // ref = -inf: nothing but -inf and NaN so far; E = NaN then, and for a far reference
+    __device__ __forceinline__ void init() { ref = -INFINITY; E = NAN; s = 0.0f; }
     __device__ __forceinline__ void refer(float high) {
         ref = high;
-        M = fabsf(ref) < kFar ? ref * kLog2e : NAN;
+        E = near(ref) ? base_of(ref) : NAN;
     }
     static __device__ __noinline__ FixedSum careful(FixedSum f, uint4 raw) {
         VecMax<T> top;
         top.add(raw);
         const float high = top.get();
         if (high > f.ref) {
-            const float r = f.out(f.s) * ex2((f.ref - high) * kLog2e);     // 0 * 0 at the start
+            f.s *= rebase(f.ref, high);     // 0 * 0 at the start
             f.refer(high);
-            f.s = f.in(r);
         }
         float t = 0.0f, v[N];
         Elem<T>::unpack(raw, v);
 #pragma unroll
-        for (int i = 0; i < N; ++i) t += f.ref == -INFINITY ? (v[i] != v[i] ? NAN : 0.0f) : ex2((v[i] - f.ref) * kLog2e);
-        f.s += f.in(t);
+        for (int i = 0; i < N; ++i) {
+            if (f.E == f.E) t += ex2(fmaf(v[i], kRest, fmaf(v[i], kStep, -f.E)));
+            else t += f.ref == -INFINITY ? (v[i] != v[i] ? NAN : 0.0f) : ex2((v[i] - f.ref) * kLog2e);
+        }
+        f.s += t;
         return f;
     }
-    template <int VECS>
-    __device__ __forceinline__ void add(const uint4 (&raw)[VECS], bool first = false) {
+    // `first`: this thread's first step, which the lanes of `mask()` take together
+    template <int VECS, class Mask>
+    __device__ __forceinline__ void add(const uint4 (&raw)[VECS], bool first, const Mask& mask) {
         if (first) {
             VecMax<T> top;
 #pragma unroll
             for (int u = 0; u < VECS; ++u) top.add(raw[u]);
-            refer(top.get());
+            refer(lanes_max(top.get(), mask()));
         }
         unsigned long long t2 = 0;
 #pragma unroll
         for (int u = 0; u < VECS; ++u) {
             float v[N];
             Elem<T>::unpack(raw[u], v);
-            exps_fma(v, M);
+            exps_fine(v, E);
 #pragma unroll
             for (int i = 0; i < N; i += 2) t2 = add2(t2, bits_of(v[i], v[i + 1]));
         }
         const Two h = two_of(t2);
         const float t = h.a + h.b;
-        if (t < 1.1529215e18f) {
+        if (t < 2.0f) {
             s += t;
         } else {
 #pragma unroll
@@ -534,7 +581,7 @@ __device__ __forceinline__ void join_warp(float& s, float& m) {
     const float own = m;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, d));
-    s = warp_add(own == -INFINITY ? s : s * ex2((own - m) * kLog2e));     // -inf: 0, or NaN for a NaN
+    s = warp_add(s * rebase(own, m));
 }
 
 constexpr int kRowThreads = 512;
@@ -564,6 +611,7 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
     __shared__ float red_s[kRowThreads / 32], red_m[kRowThreads / 32];
     __shared__ float2 pair[kRowCluster];     // (sum, reference) of every CTA of the cluster
     __shared__ RowGrad sh;
+    __shared__ PolicyToken token;            // of thread 0 alone
     __shared__ int skipped[kRowThreads / 32];   // the place of the token's entry in its vector, for every warp
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nthr = blockDim.x;
     cg::cluster_group cluster = cg::this_cluster();
@@ -597,11 +645,10 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
     if (C > 1) cluster_arrive();
     const T* p = in.x + (long long)a * in.s0 + (long long)b * in.s1;
     const Part<T> part(p, in.vocab, rank, C);
-    PolicyToken token{};
     float at_label = 0.0f;
     if (tid == 0) {
-        if (POLICY) token = policy_token(terms, a, b, weight);
-        at_label = label < in.vocab ? Elem<T>::get(*TPB_CK(&p[label])) : 0.0f;
+        if (POLICY) fetch_token(terms, a, b, weight, &token);
+        if (label < in.vocab) at_label = Elem<T>::get(*TPB_CK(&p[label]));
     }
     const int edge = part.edge(tid, in.vocab, rank, C);
     const float edge_x = edge >= 0 ? Elem<T>::get(*TPB_CK(&p[edge])) : -INFINITY;
@@ -617,27 +664,30 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
     {
         // a row that is swept twice stays in L2 until then
         const unsigned long long policy = POLICY && o ? l2_last() : l2_first();
+        // the lanes of this warp whose first step has two vectors, or one
+        const auto pairs = [&] { return lanes_below(part.n - nthr - (tid & ~31)); };
+        const auto singles = [&] { return lanes_below(part.n - (tid & ~31)) & ~pairs(); };
         int i = tid;
         for (; i + nthr < part.n; i += 2 * nthr) {
             uint4 raw[2] = {ld_policy16(q + (size_t)i * N, policy), ld_policy16(q + (size_t)(i + nthr) * N, policy)};
             const int d = skip - i;
             if (d == 0 || d == nthr) leave_out<T>(raw, (d == 0 ? 0 : N) + skipped[warp]);
-            sum.add(raw, i == tid);
+            sum.add(raw, i == tid, pairs);
         }
         if (i < part.n) {
             uint4 raw[1] = {ld_policy16(q + (size_t)i * N, policy)};
             if (i == skip) leave_out<T>(raw, skipped[warp]);
-            sum.add(raw, i == tid);
+            sum.add(raw, i == tid, singles);
         }
         if (edge >= 0 && edge != at) {      // as a vector with one element
             float v[N];
 #pragma unroll
             for (int e = 0; e < N; ++e) v[e] = e == 0 ? edge_x : -INFINITY;
             const uint4 raw[1] = {Elem<T>::pack(v)};
-            sum.add(raw);
+            sum.add(raw, false, [] { return 0u; });
         }
     }
-    float m = sum.ref, s = sum.out(sum.s);
+    float m = sum.ref, s = sum.s;
     join_warp(s, m);
     if (nthr > 32) {
         if (lane == 0) {
@@ -645,23 +695,28 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
             red_m[warp] = m;
         }
         __syncthreads();
-        const int nw = nthr >> 5;
-        s = lane < nw ? red_s[lane] : 0.0f;
-        m = lane < nw ? red_m[lane] : -INFINITY;
-        join_warp(s, m);
+        if (warp == 0) {                    // the others have no use for the sum
+            const int nw = nthr >> 5;
+            s = lane < nw ? red_s[lane] : 0.0f;
+            m = lane < nw ? red_m[lane] : -INFINITY;
+            join_warp(s, m);
+        }
     }
     if (C > 1) {
         cluster_wait();                     // all CTAs of the cluster have started
         if (tid < C) *cluster.map_shared_rank(&pair[rank], (unsigned)tid) = make_float2(s, m);
         cluster.sync();
-        const float2 v = lane < C ? pair[lane & (kRowCluster - 1)] : make_float2(0.0f, -INFINITY);
-        s = v.x;
-        m = v.y;
-        join_warp(s, m);                    // the same order in every CTA
+        if (warp == 0) {
+            const float2 v = lane < C ? pair[lane & (kRowCluster - 1)] : make_float2(0.0f, -INFINITY);
+            s = v.x;
+            m = v.y;
+            join_warp(s, m);                // the same order in every CTA
+        }
     }
     if (tid == 0) {
         const Score y = score_of(at >= 0, at_label, m, s);
         if (POLICY) {
+            asm volatile("cp.async.wait_all;" ::: "memory");
             const PolicyRow row = policy_row(terms, token, y.logp);
             const float2 k = unit_of(y, at_label, m, s);
             sh.set(k.x, k.y, y.rest(), row.coef, at);
@@ -713,8 +768,9 @@ score_grad_kernel(Logits<T> in, PerToken<long long> labels, PerToken<float> grad
         const float2 k = *TPB_CK(&keep[r]);
         g.set(k.x, k.y, -expm1f(*TPB_CK(&logp[r])), coef, at);
     } else {
-        const float n = *TPB_CK(&lse[r]);      // p = 2^(c (x - lse))
-        g.set(n, 1.0f, -expm1f(y < in.vocab ? (float)((double)Elem<T>::get(*TPB_CK(&p[y])) - (double)n) : NAN), coef, at);
+        const float n = *TPB_CK(&lse[r]);      // p = 2^(c x - E) 2^(E - c lse)
+        const float unit = near(n) ? ex2(fmaf(n, -kLog2e, base_of(n)) - n * (float)(1.4426950408889634 - (double)kLog2e)) : 1.0f;
+        g.set(n, unit, -expm1f(y < in.vocab ? (float)((double)Elem<T>::get(*TPB_CK(&p[y])) - (double)n) : NAN), coef, at);
     }
     if (y >= in.vocab) g.k = NAN;
     grad_part(p, o, part, g, edge, edge_x);

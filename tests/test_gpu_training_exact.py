@@ -223,3 +223,33 @@ def test_tokens_with_a_probability_near_one(cuda, tpb, dtype, vocab, shift):
     slope = -1024.0 * 0.5 * torch.sigmoid(-(m[0::2] - m[1::2])) / (n // 2)
     g = grad_rows(x[:n], lab[:n], torch.stack([slope, -slope], 1).flatten())
     close(grad, g, g.abs() * (3 * R.P + 2.0 ** -19 + u(dtype)) + R.TINY[dtype], "gradient of preference_loss")
+
+
+@EACH
+@pytest.mark.parametrize("rows,vocab,spread,offset", [(2048, 32000, 2.0, 0.0), (512, 151936, 2.0, 0.0), (2048, 1000, 2.0, 0.0), (2048, 32000, 1.0, 40.0), (2048, 50021, 3.0, -12.0)])
+def test_sums_are_not_off_to_one_side(cuda, tpb, dtype, rows, vocab, spread, offset):
+    """The mean error of the float64 log-probabilities that a reward adds up (ref = the right value, rounded, so that the reward
+    is small and its float32 holds it).  One row: roundings of 2^-22 and ex2's 1.5e-7, of either sign, averaged over its
+    terms: at most 1.5e-7, over the rows 1.5e-7 / sqrt(rows) a standard deviation.  Equal logits have equal errors in every
+    row, and 16-bit logits are equal often (near 40 a bfloat16 has four values to 1, and a row some twenty in all): with w_k
+    the mean share of the value k, the errors of the values are independent, so that their mean has a standard deviation of
+    1.5e-7 sqrt(sum of w_k^2), however many rows there are.  Four of both.  To one side: 1e-10 of the base; the
+    arguments of ex2 are below 1, and 8.4e-8 (the difference of ex2's mean errors on either side of zero) count for
+    the share of the sum above E, under 0.15: 1.3e-8."""
+    g = torch.Generator(device=cuda).manual_seed(rows + vocab)
+    x = (torch.randn(rows, vocab, device=cuda, generator=g) * spread + offset).to(dtype)
+    lab = labels_of(cuda, (rows,), vocab, 5)
+    want = torch.cat([exact_rows(x[i:i + 256], lab[i:i + 256])[0] for i in range(0, rows, 256)])
+    ref = want.float()
+    loss, _, rewards, _ = tpb.preference_loss(x, lab, ref, torch.tensor([0, rows // 2, rows], device=cuda), beta=1.0, need_grad=False)
+    off = (rewards.double().sum() - (want - ref.double()).sum()).item() / rows
+    share = 0.0
+    if dtype != torch.float32:
+        values, at = x.unique(return_inverse=True)
+        w = torch.zeros(values.numel(), dtype=torch.float64, device=cuda)
+        for i in range(0, rows, 256):
+            w.scatter_add_(0, at[i:i + 256].flatten(), exact_rows(x[i:i + 256], lab[i:i + 256])[1].flatten() / rows)
+        share = w.square().sum().sqrt().item()
+    bound = 1.3e-8 + 4 * 1.5e-7 * (rows ** -0.5 + share)
+    print(f"mean error {off:.3e}, bound {bound:.3e}")
+    assert abs(off) <= bound
