@@ -311,7 +311,9 @@ int tpb200_reduce_all_noalloc(int op, const void* in, int dtype, int64_t n, int6
  *   - The results of a call do not depend on the order in which its CTAs run: no floating-point atomics.
  *
  * tpb200_token_logprobs: logp = logits[label] - lse, lse = log sum exp(logits), of every row.
- * tpb200_token_logprobs_backward: grad_logits = grad_logp * ([j = label] - exp(logits - lse)).
+ * tpb200_token_logprobs_backward: grad_logits = grad_logp * ([j = label] - exp(logits - lse)), with lse from the
+ *   forward call.  Rows whose float32 lse does not hold the digits (|lse| of 32 and more, tokens with half of the
+ *   probability and more) are summed again.
  *   A row with a negative label takes no part: it is not read, logp = lse = 0, its gradient is zero.  A
  *   label of `vocab` or more gives NaN for its row (no access outside the row is made).  -inf logits have
  *   probability 0; NaN, +inf and all -inf rows give NaN as log_softmax does.

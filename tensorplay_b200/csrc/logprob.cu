@@ -576,6 +576,12 @@ struct ScoreOut {
     float* coef;         // set to zero: rows of no sequence keep that
 };
 
+// The gradient of logp that the caller has, and lse as the forward call rounded it.
+struct BackwardIn {
+    PerToken<float> grad;
+    const float* lse;
+};
+
 // (sum, reference) pairs of the lanes as one
 __device__ __forceinline__ void join_warp(float& s, float& m) {
     const float own = m;
@@ -592,7 +598,7 @@ constexpr int kRowCtas = 4;
 #endif
 constexpr int kRowCluster = 8;
 
-// Log-probabilities, and with POLICY the whole policy loss: a cluster of C CTAs per row, each with 1/C of the
+// Log-probabilities, the whole policy loss, or the gradient of log-probabilities: a cluster of C CTAs per row, each with 1/C of the
 // row's 16-byte vectors.  The first sweep sums, the CTAs' (sum, reference) pairs cross the cluster through
 // distributed shared memory, and the second sweep writes the gradient; it reads the row again, from L2,
 // because C is chosen so that the rows in flight take half of it (row_shape), and because loads and stores say
@@ -603,11 +609,13 @@ constexpr int kRowCluster = 8;
 // f32 4.83 (C = 6); with two CTAs of 512 on an SM instead of four 4.0, 4.0 and 4.3; in separate kernels for
 // sum and gradient 3.8 and 3.8.  Keeping the row in shared memory instead (a ring of bulk copies, persistent CTAs)
 // left 16 to 26 warps on an SM to hide the latencies and was slower: 4.6, 4.0 and 3.2.
-template <class T, bool POLICY>
+enum Mode { kScores, kPolicy, kBackward };
+template <class T, int MODE>
 __global__ void __launch_bounds__(kRowThreads, kRowCtas)
-row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTerms terms, PolicyOut out, ScoreOut score, T* __restrict__ grad, int C,
-           float* __restrict__ loss) {
+row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTerms terms, PolicyOut out, ScoreOut score, BackwardIn back,
+           T* __restrict__ grad, int C, float* __restrict__ loss) {
     constexpr int N = Elem<T>::N;
+    constexpr bool POLICY = MODE == kPolicy, BACKWARD = MODE == kBackward;
     __shared__ float red_s[kRowThreads / 32], red_m[kRowThreads / 32];
     __shared__ float2 pair[kRowCluster];     // (sum, reference) of every CTA of the cluster
     __shared__ RowGrad sh;
@@ -618,16 +626,16 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
     const int rank = C > 1 ? (int)cluster.block_rank() : 0;
     const unsigned r = blockIdx.x / (unsigned)C, a = r / (unsigned)in.inner, b = r - a * (unsigned)in.inner;
     long long label = labels.at(a, b);
-    float weight = 0.0f;
-    if (POLICY) {
-        weight = terms.weight.at(a, b);
+    float weight = 0.0f;                    // BACKWARD: the caller's gradient of logp
+    if (POLICY || BACKWARD) {
+        weight = POLICY ? terms.weight.at(a, b) : back.grad.at(a, b);
         if (weight == 0.0f) label = -1;
     } else if (!limits.inside(r)) {
         label = -1;
     }
-    T* o = POLICY && grad ? grad + (long long)r * in.vocab : nullptr;
+    T* o = MODE != kScores && grad ? grad + (long long)r * in.vocab : nullptr;
     if (label < 0) {
-        if (tid == 0 && rank == 0) {
+        if (!BACKWARD && tid == 0 && rank == 0) {
             if (POLICY) {
                 store_policy(out, r, 0.0, PolicyRow{0.0f, 0.0f, 0.0f, 0.0});
                 if (loss) *TPB_CK(loss) = 0.0f;
@@ -639,22 +647,36 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
                 if (score.coef) *TPB_CK(&score.coef[r]) = 0.0f;
             }
         }
-        if (POLICY && o) zero_part(o, Part<T>(o, in.vocab, rank, C), in.vocab, rank, C);
+        if (MODE != kScores && o) zero_part(o, Part<T>(o, in.vocab, rank, C), in.vocab, rank, C);
         return;                             // all CTAs of the cluster alike
     }
-    if (C > 1) cluster_arrive();
     const T* p = in.x + (long long)a * in.s0 + (long long)b * in.s1;
     const Part<T> part(p, in.vocab, rank, C);
-    float at_label = 0.0f;
-    if (tid == 0) {
-        if (POLICY) fetch_token(terms, a, b, weight, &token);
-        if (label < in.vocab) at_label = Elem<T>::get(*TPB_CK(&p[label]));
-    }
+    const int at = label < in.vocab ? (int)label : -1;
     const int edge = part.edge(tid, in.vocab, rank, C);
     const float edge_x = edge >= 0 ? Elem<T>::get(*TPB_CK(&p[edge])) : -INFINITY;
+    float at_label = 0.0f;
+    if (BACKWARD) {
+        if (at >= 0) at_label = Elem<T>::get(*TPB_CK(&p[at]));
+        const float lse = *TPB_CK(&back.lse[r]);
+        // The float32 lse is up to 2^-24 |lse| off, and so is every p.  It serves while that is under 2^-20 and the token has
+        // less than half of the probability (it goes by 1 - p); else the row is summed again (all CTAs alike).
+        if (at < 0 || (fabsf(lse) < 32.0f && at_label - lse < -0.7f)) {
+            RowGrad g;
+            // p = 2^(c x - E) 2^(E - c lse)
+            const float unit = ex2(fmaf(lse, -kLog2e, base_of(lse)) - lse * (float)(1.4426950408889634 - (double)kLog2e));
+            g.set(lse, unit, at < 0 ? NAN : -expm1f((float)((double)at_label - (double)lse)), weight, at);
+            if (at < 0) g.k = NAN;
+            grad_part(p, o, part, g, edge, edge_x);
+            return;
+        }
+    } else if (tid == 0) {
+        if (POLICY) fetch_token(terms, a, b, weight, &token);
+        if (at >= 0) at_label = Elem<T>::get(*TPB_CK(&p[at]));
+    }
+    if (C > 1) cluster_arrive();
 
     // ---- the sum of all but the token's own term
-    const int at = label < in.vocab ? (int)label : -1;
     const int skip = at >= part.head && at < in.vocab - part.tail ? (at - part.head) / N - part.first : -1;   // the vector with the token's entry
     if (lane == 0) skipped[warp] = (at - part.head) & (N - 1);
     __syncwarp();
@@ -663,7 +685,7 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
     sum.init();
     {
         // a row that is swept twice stays in L2 until then
-        const unsigned long long policy = POLICY && o ? l2_last() : l2_first();
+        const unsigned long long policy = MODE != kScores && o ? l2_last() : l2_first();
         // the lanes of this warp whose first step has two vectors, or one
         const auto pairs = [&] { return lanes_below(part.n - nthr - (tid & ~31)); };
         const auto singles = [&] { return lanes_below(part.n - (tid & ~31)) & ~pairs(); };
@@ -724,6 +746,9 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
                 store_policy(out, r, y.logp, row);
                 if (loss) *TPB_CK(loss) = (float)row.part;
             }
+        } else if (BACKWARD) {
+            const float2 k = unit_of(y, at_label, m, s);
+            sh.set(k.x, k.y, y.rest(), weight, at);
         } else if (rank == 0) {
             *TPB_CK(&score.logp[r]) = (float)y.logp;
             if (score.lse) *TPB_CK(&score.lse[r]) = (float)y.lse;
@@ -732,28 +757,26 @@ row_kernel(Logits<T> in, PerToken<long long> labels, RowLimits limits, PolicyTer
             if (score.coef) *TPB_CK(&score.coef[r]) = 0.0f;
         }
     }
-    if (!POLICY || !o) return;
+    if (MODE == kScores || !o) return;
     __syncthreads();
     const RowGrad g = sh;
     grad_part(p, o, part, g, edge, edge_x);
 }
 
 // ---------------------------------------------------------------- gradient from saved statistics
-// coef of every row from the caller's grad_logp (with lse), or from a workspace (with keep).
+// The preference loss's second part, by the (reference, unit) of every row and its coefficient.
 template <class T>
 __global__ void __launch_bounds__(kRowThreads, kRowCtas)
-score_grad_kernel(Logits<T> in, PerToken<long long> labels, PerToken<float> grad_logp, const float* __restrict__ lse,
-                  const float2* __restrict__ keep, const float* __restrict__ coefs, const float* __restrict__ logp, T* __restrict__ out, unsigned rows,
-                  int C, PairSum sum) {
+score_grad_kernel(Logits<T> in, PerToken<long long> labels, const float2* __restrict__ keep, const float* __restrict__ coefs,
+                  const float* __restrict__ logp, T* __restrict__ out, unsigned rows, int C, PairSum sum) {
     if (blockIdx.x == 0) sum.run();
-    // with saved statistics the rows go backwards: the last ones that the sums read are still in L2
-    unsigned r = blockIdx.x / (unsigned)C;
-    const int rank = (int)(blockIdx.x - r * (unsigned)C);
-    if (keep) r = rows - 1 - r;
+    // the rows go backwards: the last ones that the sums read are still in L2
+    const unsigned from = blockIdx.x / (unsigned)C, r = rows - 1 - from;
+    const int rank = (int)(blockIdx.x - from * (unsigned)C);
     const unsigned a = r / (unsigned)in.inner, b = r - a * (unsigned)in.inner;
     T* o = out + (long long)r * in.vocab;
     const long long y = labels.at(a, b);
-    const float coef = y < 0 ? 0.0f : (coefs ? *TPB_CK(&coefs[r]) : grad_logp.at(a, b));
+    const float coef = y < 0 ? 0.0f : *TPB_CK(&coefs[r]);
     if (coef == 0.0f) {
         zero_part(o, Part<T>(o, in.vocab, rank, C), in.vocab, rank, C);
         return;
@@ -763,15 +786,8 @@ score_grad_kernel(Logits<T> in, PerToken<long long> labels, PerToken<float> grad
     const int edge = part.edge(threadIdx.x, in.vocab, rank, C);
     const float edge_x = edge >= 0 ? Elem<T>::get(*TPB_CK(&p[edge])) : -INFINITY;
     RowGrad g;
-    const int at = y < in.vocab ? (int)y : -1;
-    if (keep) {
-        const float2 k = *TPB_CK(&keep[r]);
-        g.set(k.x, k.y, -expm1f(*TPB_CK(&logp[r])), coef, at);
-    } else {
-        const float n = *TPB_CK(&lse[r]);      // p = 2^(c x - E) 2^(E - c lse)
-        const float unit = near(n) ? ex2(fmaf(n, -kLog2e, base_of(n)) - n * (float)(1.4426950408889634 - (double)kLog2e)) : 1.0f;
-        g.set(n, unit, -expm1f(y < in.vocab ? (float)((double)Elem<T>::get(*TPB_CK(&p[y])) - (double)n) : NAN), coef, at);
-    }
+    const float2 k = *TPB_CK(&keep[r]);
+    g.set(k.x, k.y, -expm1f(*TPB_CK(&logp[r])), coef, y < in.vocab ? (int)y : -1);
     if (y >= in.vocab) g.k = NAN;
     grad_part(p, o, part, g, edge, edge_x);
 }
@@ -885,25 +901,25 @@ inline RowShape row_shape(int64_t rows, int64_t vocab, int64_t elem, bool twice)
     return s;
 }
 
-template <class T, bool POLICY>
+template <class T, int MODE>
 int row_run(const Logits<T>& in, const PerToken<long long>& lab, const RowLimits& limits, const PolicyTerms& terms, const PolicyOut& out,
-            const ScoreOut& score, T* grad, int64_t rows, float* loss, cudaStream_t st) {
+            const ScoreOut& score, const BackwardIn& back, T* grad, int64_t rows, float* loss, cudaStream_t st) {
     const RowShape s = row_shape(rows, in.vocab, sizeof(T), grad != nullptr);
-    const cudaError_t e = launch_ex(row_kernel<T, POLICY>, dim3((unsigned)(rows * s.C)), s.threads, 0, st, s.C, false, in, lab, limits, terms, out, score, grad,
-                                    s.C, rows == 1 ? loss : nullptr);
+    const cudaError_t e = launch_ex(row_kernel<T, MODE>, dim3((unsigned)(rows * s.C)), s.threads, 0, st, s.C, false, in, lab, limits, terms, out, score, back,
+                                    grad, s.C, rows == 1 ? loss : nullptr);
     return e == cudaSuccess ? TPB200_OK : cuda_fail(e, "row_kernel");
 }
 template <class T>
 int score_run(const Logits<T>& in, const PerToken<long long>& lab, const RowLimits& limits, float* logp, float* lse, float2* keep,
               double* exact, float* coef, int64_t rows, cudaStream_t st) {
-    return row_run<T, false>(in, lab, limits, PolicyTerms{}, PolicyOut{}, ScoreOut{logp, lse, keep, exact, coef}, (T*)nullptr, rows, nullptr, st);
+    return row_run<T, kScores>(in, lab, limits, PolicyTerms{}, PolicyOut{}, ScoreOut{logp, lse, keep, exact, coef}, BackwardIn{}, (T*)nullptr, rows, nullptr, st);
 }
 template <class T>
-int score_grad_run(const Logits<T>& in, const PerToken<long long>& lab, const PerToken<float>& grad_logp, const float* lse, const float2* keep,
-                   const float* coefs, const float* logp, T* out, int64_t rows, const PairSum& sum, cudaStream_t st) {
+int score_grad_run(const Logits<T>& in, const PerToken<long long>& lab, const float2* keep, const float* coefs, const float* logp, T* out,
+                   int64_t rows, const PairSum& sum, cudaStream_t st) {
     const RowShape s = row_shape(rows, in.vocab, sizeof(T), false);
-    TPB_LAUNCH("score_grad_kernel", score_grad_kernel<T>, dim3((unsigned)(rows * s.C)), s.threads, 0, st, in, lab, grad_logp, lse, keep, coefs, logp, out,
-               (unsigned)rows, s.C, sum);
+    TPB_LAUNCH("score_grad_kernel", score_grad_kernel<T>, dim3((unsigned)(rows * s.C)), s.threads, 0, st, in, lab, keep, coefs, logp, out, (unsigned)rows,
+               s.C, sum);
     return TPB200_OK;
 }
 
@@ -952,8 +968,9 @@ extern "C" int tpb200_token_logprobs_backward(const float* grad_logp, const int6
                      rows_range(grad_logp, outer, inner, 1, grad_strides, 4), HostRange{lse, (size_t)rows * 4},
                      HostRange{grad_logits, (size_t)(rows * vocab * dtype_bytes(dtype))});
     const PerToken<long long> lab{(const long long*)labels, label_strides[0], label_strides[1]};
-    TPB_BY_TYPE(dtype, return score_grad_run<T>(logits_of<T>(logits, inner, vocab, strides), lab, per_token(grad_logp, grad_strides), lse, nullptr, nullptr,
-                                                nullptr, (T*)grad_logits, rows, PairSum{}, st));
+    const BackwardIn back{per_token(grad_logp, grad_strides), lse};
+    TPB_BY_TYPE(dtype, return (row_run<T, kBackward>(logits_of<T>(logits, inner, vocab, strides), lab, RowLimits{nullptr, 0}, PolicyTerms{}, PolicyOut{},
+                                                     ScoreOut{}, back, (T*)grad_logits, rows, nullptr, st)));
     return TPB200_OK;
 }
 
@@ -993,8 +1010,8 @@ extern "C" int tpb200_policy_loss(const void* logits, int dtype, int64_t outer, 
         const PolicyTerms terms{per_token(old_logp, old_strides), per_token(advantages, advantage_strides), per_token(weights, weight_strides),
                                 per_token(ref_logp, ref_strides), (float)clip_low, (float)clip_high, (float)kl_coef, (float)grad_scale};
         const PolicyOut out{logp, ratio, kl, (double*)workspace};
-        TPB_BY_TYPE(dtype, rc = (row_run<T, true>(logits_of<T>(logits, inner, vocab, strides), lab, RowLimits{nullptr, 0}, terms, out,
-                                                  ScoreOut{}, (T*)grad_logits, rows, loss, st)));
+        TPB_BY_TYPE(dtype, rc = (row_run<T, kPolicy>(logits_of<T>(logits, inner, vocab, strides), lab, RowLimits{nullptr, 0}, terms, out,
+                                                  ScoreOut{}, BackwardIn{}, (T*)grad_logits, rows, loss, st)));
         if (rc != TPB200_OK || rows == 1) return rc;     // a single row has written the loss itself
     }
     TPB_LAUNCH("loss_sum_kernel", loss_sum_kernel, dim3(1), 1024, 0, st, (const double*)workspace, (long long)rows, 1.0, loss);
@@ -1047,7 +1064,6 @@ extern "C" int tpb200_preference_loss(const void* logits, int dtype, int64_t out
     if (!few) TPB_LAUNCH("loss_sum_kernel", loss_sum_kernel, dim3(1), 1024, 0, st, (const double*)part, (long long)pairs, 1.0 / (double)pairs, loss);
     else if (!beside) TPB_LAUNCH("pair_sum_kernel", pair_sum_kernel, dim3(1), 32, 0, st, sum);
     if (rows > 0 && grad_logits)
-        TPB_BY_TYPE(dtype, return score_grad_run<T>(logits_of<T>(logits, inner, vocab, strides), lab, PerToken<float>{nullptr, 0, 0}, nullptr, keep, coefs,
-                                                    logp, (T*)grad_logits, rows, beside ? sum : PairSum{}, st));
+        TPB_BY_TYPE(dtype, return score_grad_run<T>(logits_of<T>(logits, inner, vocab, strides), lab, keep, coefs, logp, (T*)grad_logits, rows, beside ? sum : PairSum{}, st));
     return TPB200_OK;
 }

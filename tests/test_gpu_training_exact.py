@@ -253,3 +253,23 @@ def test_sums_are_not_off_to_one_side(cuda, tpb, dtype, rows, vocab, spread, off
     bound = 1.3e-8 + 4 * 1.5e-7 * (rows ** -0.5 + share)
     print(f"mean error {off:.3e}, bound {bound:.3e}")
     assert abs(off) <= bound
+
+
+@EACH
+@pytest.mark.parametrize("vocab", [2, 77, 8191, 32000, 50021])
+def test_gradient_of_log_probabilities_where_lse_does_not_hold_them(cuda, tpb, dtype, vocab):
+    """The separate backward call has lse as a float32 alone.  Rows whose token has nearly all of the probability, rows around
+    large values, and logits with a large common part lose digits there: they are held to the bounds of the losses
+    that have the sums (P twice, 2^-19).  Where lse serves, |lse| < 32, it costs p 2^-20 of itself."""
+    x, lab = confident(cuda, dtype, vocab, 3 + vocab)
+    far, at = far_rows(cuda, dtype, vocab)
+    off = logits_of(cuda, (6, vocab), torch.float32, 5) + torch.tensor([31.0, -40.0, 500.0, -3000.0, 5000.0, 2e4], device=cuda).unsqueeze(1)
+    x = torch.cat([x, far, off.to(dtype), logits_of(cuda, (40, vocab), dtype, 9, spread=6.0)])
+    lab = torch.cat([lab, at.clamp_max(vocab - 1), labels_of(cuda, (46,), vocab, 6)])
+    coef = torch.randn(lab.numel(), device=cuda, generator=torch.Generator(device=cuda).manual_seed(1)) * 8
+    coef[::11] = 0.0
+    logp, lse = tpb.token_logprobs(x, lab)
+    for rows in (slice(None), slice(0, 1), slice(-46, None)):
+        g = tpb.token_logprobs_backward(coef[rows], x[rows], lab[rows], lse[rows])
+        want = grad_rows(x[rows], lab[rows], coef[rows])
+        close(g, want, want.abs() * (2 * R.P + 2.0 ** -19 + u(dtype)) + R.TINY[dtype], "grad_logits")
