@@ -302,7 +302,8 @@ __device__ __forceinline__ float kl_term(float d) {
         t = fmaf(t, d, 0.5f);
         return t * d * d;
     }
-    return expm1f(d) - d;
+    const float e = expm1f(d);
+    return e == INFINITY ? e : e - d;     // inf - inf at d = inf
 }
 
 // A token's inputs, fetched before the row is swept, asynchronously into shared memory: the sweep has no register to
@@ -334,8 +335,10 @@ __device__ __forceinline__ PolicyRow policy_row(const PolicyTerms& t, const Poli
     if (t.ref.p) {
         const float d = (float)((double)k.ref - logp);
         o.kl = kl_term(d);
-        loss = fmaf(t.kl_coef, o.kl, loss);
-        slope = fmaf(t.kl_coef, -expm1f(d), slope);
+        if (t.kl_coef > 0.0f) {                  // 0 * inf must not appear: a KL that is only watched may be infinite
+            loss = fmaf(t.kl_coef, o.kl, loss);
+            slope = fmaf(t.kl_coef, -expm1f(d), slope);
+        }
     }
     o.part = (double)k.weight * (double)loss;
     o.coef = k.weight * slope * t.grad_scale;

@@ -273,3 +273,23 @@ def test_gradient_of_log_probabilities_where_lse_does_not_hold_them(cuda, tpb, d
         g = tpb.token_logprobs_backward(coef[rows], x[rows], lab[rows], lse[rows])
         want = grad_rows(x[rows], lab[rows], coef[rows])
         close(g, want, want.abs() * (2 * R.P + 2.0 ** -19 + u(dtype)) + R.TINY[dtype], "grad_logits")
+
+
+@EACH
+def test_an_infinite_kl_that_is_only_watched(cuda, tpb, dtype):
+    """With kl_coef = 0 the KL term is reported, and is no part of the loss or of the gradient, whatever it is."""
+    x, lab, old, adv, w, ref = policy_inputs(cuda, (7,), 301, dtype, 12, masked=0.0)
+    plain = tpb.policy_loss(x, lab, old, adv, w, kl_coef=0.0)
+    ref = ref.clone()
+    ref[1], ref[2] = float("-inf"), 200.0                   # kl = inf - ... at d = -inf, e^d beyond float32 at d > 200
+    loss, grad, logp, ratio, kl = tpb.policy_loss(x, lab, old, adv, w, ref, kl_coef=0.0)
+    assert bool(kl[1:3].isinf().all()) and bool(kl[[0, 3, 4, 5, 6]].isfinite().all())
+    for a, b in zip((loss, grad, logp, ratio), plain):
+        assert torch.equal(a, b)
+    x = x.clone()
+    x[3, lab[3]] = float("-inf")                            # a token that a mask has taken out: logp = -inf, ratio 0, kl infinite
+    loss, grad, logp, ratio, kl = tpb.policy_loss(x, lab, old, adv, w, ref, kl_coef=0.0)
+    assert logp[3] == float("-inf") and ratio[3] == 0 and kl[3] == float("inf")
+    assert bool(loss.isfinite()) and bool((grad[3] == 0).all()) and bool(grad.isfinite().all())
+    # counted, it is an infinite loss
+    assert bool(tpb.policy_loss(x, lab, old, adv, w, ref, kl_coef=0.1)[0].isinf())
