@@ -3,7 +3,9 @@
 #include "common.cuh"
 #include "host_util.h"
 
+#include <map>
 #include <mutex>
+#include <utility>
 
 namespace tpb {
 
@@ -35,6 +37,20 @@ int sm_count() {
         cached[dev] = n;
     }
     return cached[dev];
+}
+
+int allow_shared(const void* kernel, size_t bytes) {
+    if (bytes + 8192 <= 48 * 1024) return TPB200_OK;      // static shared memory counts against the 48 KB default too
+    static std::mutex mu;
+    static std::map<std::pair<int, const void*>, size_t> granted;
+    int dev = 0;
+    TPB_CUDA_OK(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lk(mu);
+    size_t& most = granted[{dev, kernel}];
+    if (bytes <= most) return TPB200_OK;
+    TPB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    most = bytes;
+    return TPB200_OK;
 }
 
 // Set by a kernel whose bounded wait gave up (its outputs are then not written): top-k rendezvous /

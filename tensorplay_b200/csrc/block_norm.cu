@@ -768,7 +768,8 @@ int forward_run(const ForwardArgs<T>& k, cudaStream_t st) {
     if (vec && k.width > 256 && k.width <= 8192) {
         const int threads = staged_threads(k.width);
         const size_t smem = (size_t)threads * kStages * kForwardArrays * 8 * sizeof(T);
-        TPB_CUDA_OK(cudaFuncSetAttribute(block_forward_staged_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        const int rc = allow_shared((const void*)block_forward_staged_kernel<T>, smem);
+        if (rc != TPB200_OK) return rc;
         const long long ctas = std::min<long long>(k.rows, (long long)sm_count() * resident_ctas(threads, 2048, smem));
         TPB_LAUNCH("block_forward_staged_kernel", block_forward_staged_kernel<T>, dim3((unsigned)ctas), threads, smem, st, k);
         return TPB200_OK;
@@ -792,7 +793,8 @@ int backward_run(const BackwardArgs<T>& k, T* dpost, T* dnext, long long gate_gr
         const bool sums = k.gate.p && !k.gate_rows;
         const auto kernel = k.from_x ? (sums ? block_backward_staged_kernel<T, true, true> : block_backward_staged_kernel<T, false, true>)
                                      : (sums ? block_backward_staged_kernel<T, true, false> : block_backward_staged_kernel<T, false, false>);
-        TPB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        const int rc = allow_shared((const void*)kernel, smem);
+        if (rc != TPB200_OK) return rc;
         TPB_LAUNCH("block_backward_staged_kernel", kernel, dim3((unsigned)k.workers), threads, smem, st, k);
     } else {
         TPB_BLOCK_LAUNCH(block_backward_kernel, T, p, grid, mask_bytes(p, k.width, k.drop), st, k);

@@ -45,6 +45,10 @@ inline int cuda_fail(cudaError_t e, const char* what) {
     } while (0)
 
 int sm_count();  // SMs of the current device (148 on B200), cached per device
+// Lets launches of `kernel` on the current device take `bytes` of dynamic shared memory.  The limit belongs to the function on
+// the device, for all host threads: it is only ever raised, so that a thread with a small launch cannot take away
+// what another one has just been granted, and a call that it covers already makes no driver call.
+int allow_shared(const void* kernel, size_t bytes);
 int* device_status_word();  // device address of the per-device status word (nullptr without a device)
 
 // Planner overrides for experiments and tests (TPB200_FORCE_STRATEGY, TPB200_TOPK_SLICES, ...) are

@@ -463,8 +463,8 @@ extern "C" int tpb200_softmax(int log, const void* in, int dtype, int ndim, cons
         cudaError_t e = cudaSuccess;
 #define TPB_SM_LONG(LOGV, STAGEV)                                                                                  \
     do {                                                                                                           \
-        if (smem + 8192 > 48 * 1024)                                                                               \
-            TPB_CUDA_OK(cudaFuncSetAttribute(softmax_long_kernel<LOGV, STAGEV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); \
+        const int rc = allow_shared((const void*)softmax_long_kernel<LOGV, STAGEV>, smem);                          \
+        if (rc != TPB200_OK) return rc;                                                                            \
         e = launch_ex(softmax_long_kernel<LOGV, STAGEV>, grid, threads, smem, st, S, false, x, y, k1, ks0, ks1, C, chunk, S, vec);        \
     } while (0)
         if (log) { if (stage) TPB_SM_LONG(true, true); else TPB_SM_LONG(true, false); }

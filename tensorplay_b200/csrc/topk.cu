@@ -1587,12 +1587,7 @@ static int topk_plan(const void* in, int ndim, const int64_t* sizes, const int64
 }
 
 template <class K>
-static int allow_smem(K kernel, size_t bytes) {
-    if (bytes + 8192 > 48 * 1024) {   // static shared memory counts against the 48 KB default too
-        TPB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    }
-    return TPB200_OK;
-}
+static int allow_smem(K kernel, size_t bytes) { return allow_shared((const void*)kernel, bytes); }
 
 template <bool LARGEST>
 static int select_launch(const TopkPlan& pl, const float* in, float* ov, long long* oi, cudaStream_t st) {

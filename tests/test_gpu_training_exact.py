@@ -1,6 +1,8 @@
 """GPU tests of what the training operators keep of their 64-bit formulas where digits are easily lost, and of
 calls that are rarely made.  Oracles in 64 bits; every bound is derived where it stands (u = eps / 2 is one
 rounding of the output)."""
+import threading
+
 import pytest
 import torch
 
@@ -293,3 +295,56 @@ def test_an_infinite_kl_that_is_only_watched(cuda, tpb, dtype):
     assert bool(loss.isfinite()) and bool((grad[3] == 0).all()) and bool(grad.isfinite().all())
     # counted, it is an infinite loss
     assert bool(tpb.policy_loss(x, lab, old, adv, w, ref, kl_coef=0.1)[0].isinf())
+
+
+# ------------------------------------------------------------------------------------ two host threads
+
+def both_at_once(cuda, calls, times):
+    """Every call `times` times in a host thread and on a stream of its own; what they raised, and their last results."""
+    errors, got, go = [], [None] * len(calls), threading.Barrier(len(calls))
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream(cuda)
+            s.wait_stream(torch.cuda.default_stream(cuda))
+            with torch.cuda.stream(s):
+                go.wait()
+                for _ in range(times):
+                    got[i] = calls[i]()
+            s.synchronize()
+        except Exception as e:      # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    return errors, got
+
+
+@EACH
+def test_two_host_threads_with_different_widths(cuda, tpb, dtype):
+    """The limit of a kernel's shared memory belongs to the device: a thread's narrow rows must not lower it between
+    another one's request and launch.  The calls go to the C ABI, one after the other as fast as threads make them."""
+    from tensorplay_b200 import _lib
+    L, calls, want = _lib.lib(), [], []
+    for width in (8192, 320, 4096, 288):
+        v = block_inputs(cuda, (1, 2, width), dtype, None, width)
+        want.append(tpb.block_residual(v["x"], v["h"], v["post"], v["next"]))
+        out = [torch.empty_like(t) for t in want[-1]]
+        rows = _lib.pair(0, width)
+        args = (v["x"].data_ptr(), rows, v["h"].data_ptr(), rows, None, None, v["post"].data_ptr(), v["next"].data_ptr(),
+                tpb.training._TYPES[dtype], 1, 2, width, 1.0, 1e-6, 0.0, 0, 0, *(t.data_ptr() for t in out))
+
+        def run(args=args, out=out, keep=v):
+            stream = torch.cuda.current_stream(cuda).cuda_stream
+            for _ in range(4000):
+                _lib.check(L.tpb200_block_residual(*args, stream))
+            return out
+        calls.append(run)
+    torch.cuda.synchronize()
+    errors, got = both_at_once(cuda, calls, 2)
+    assert not errors, errors[0]
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
