@@ -138,11 +138,6 @@ def _scratch(nbytes, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
-def _per_token(lead, device, count):
-    """`count` contiguous float32 outputs of shape `lead` from one allocation."""
-    return torch.empty((count, *lead), dtype=torch.float32, device=device).unbind(0)
-
-
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -217,10 +212,8 @@ def token_logprobs(logits, labels, *, out=None):
     rows, lab = _logits(logits, labels, what)
     f32 = (logits.shape[:-1], torch.float32)
     with _on(logits.device):
-        if out is None:
-            logp, lse = _per_token(logits.shape[:-1], logits.device, 2)
-        else:
-            logp, lse = _outputs(what, logits, out, [f32, f32])
+        logp, lse = _outputs(what, logits, out, [f32, f32])
+        if out is not None:
             _no_overlap(what, (logp, lse), (logits, labels))
         _lib.check(_lib.lib().tpb200_token_logprobs(*rows, *lab, logp.data_ptr(), lse.data_ptr(), _stream(logits.device)))
     return logp, lse
@@ -267,15 +260,10 @@ def policy_loss(logits, labels, old_logp, advantages, weights, ref_logp=None, *,
     f32 = (lead, torch.float32)
     with _on(device):
         nbytes = L.tpb200_policy_loss_workspace_bytes(rows[2], rows[3])
-        if out is None:
-            # one allocation for the workspace (8 bytes per token) and what comes back per token
-            ws, _, logp, ratio, kl = _per_token(lead, device, 5)
-            loss = _new((), torch.float32, ws)
-            grad = _new(logits.shape, logits.dtype, logits) if need_grad else None
-        else:
-            loss, grad, logp, ratio, kl = _outputs(what, logits, out, [((), torch.float32), (logits.shape, logits.dtype) if need_grad else None, f32, f32, f32])
+        loss, grad, logp, ratio, kl = _outputs(what, logits, out, [((), torch.float32), (logits.shape, logits.dtype) if need_grad else None, f32, f32, f32])
+        if out is not None:
             _no_overlap(what, (loss, grad, logp, ratio, kl), (logits, labels, old_logp, advantages, weights, ref_logp))
-            ws = _scratch(nbytes, device)
+        ws = _scratch(nbytes, device)
         _lib.check(L.tpb200_policy_loss(*rows, *lab, *args[0], *args[1], *args[2], *args[3], clip_low, clip_high, kl_coef, grad_scale,
                                         loss.data_ptr(), _ptr(grad), logp.data_ptr(), ratio.data_ptr(), kl.data_ptr(), _ptr(ws), nbytes,
                                         _stream(device)))

@@ -297,6 +297,23 @@ def test_an_infinite_kl_that_is_only_watched(cuda, tpb, dtype):
     assert bool(tpb.policy_loss(x, lab, old, adv, w, ref, kl_coef=0.1)[0].isinf())
 
 
+@EACH
+def test_results_are_tensors_of_their_own(cuda, tpb, dtype):
+    """No result is a view of another one or of scratch memory: keeping one keeps its own bytes, and each can be changed
+    in place in a recorded graph."""
+    x, lab, old, adv, w, ref = policy_inputs(cuda, (3, 5), 301, dtype, 12)
+    v = block_inputs(cuda, (2, 3, 64), dtype, "vector", 13)
+    x_out, y, rp, rn = block = tpb.block_residual(v["x"], v["h"], v["post"], v["next"], v["gate"])
+    results = [*tpb.token_logprobs(x, lab), *tpb.policy_loss(x, lab, old, adv, w, ref, kl_coef=0.1), *tpb.preference_loss(x[:2], lab[:2], ref[:2]), *block,
+               *tpb.block_residual_backward(v["gx"], v["gy"], v["h"], x_out, rp, rn, v["post"], v["next"], v["gate"]), *tpb.rms_norm(v["x"], v["next"])]
+    scale = torch.ones((), device=cuda, requires_grad=True)
+    for i, t in enumerate(results):
+        assert not t._is_view() and t.untyped_storage().nbytes() == t.numel() * t.element_size(), i
+        t.mul_(scale.to(t.dtype)).sum().backward()
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in results)
+    assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+
+
 # ------------------------------------------------------------------------------------ two host threads
 
 def both_at_once(cuda, calls, times):
