@@ -741,19 +741,16 @@ template <class T, class K>
 bool aligned_row(const RowView<K>& v) { return (((uintptr_t)v.p) & 15) == 0 && (v.s0 * (long long)sizeof(T)) % 16 == 0 && (v.s1 * (long long)sizeof(T)) % 16 == 0; }
 inline bool aligned16(const void* p) { return (((uintptr_t)p) & 15) == 0; }
 
-#define TPB_BLOCK_LAUNCH(KERNEL, T, plan, grid, smem, st, args)                                                                       \
-    do {                                                                                                                         \
-        if ((plan).warp) {                                                                                                       \
-            if ((plan).vec) { if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, true, true>), grid, (plan).threads, (smem), st, args);    \
-                              else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, true, true>), grid, (plan).threads, (smem), st, args); }           \
-            else            { if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, false, true>), grid, (plan).threads, (smem), st, args);   \
-                              else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, false, true>), grid, (plan).threads, (smem), st, args); }          \
-        } else {                                                                                                                 \
-            if ((plan).vec) { if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, true, false>), grid, (plan).threads, (smem), st, args);   \
-                              else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, true, false>), grid, (plan).threads, (smem), st, args); }          \
-            else            { if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, false, false>), grid, (plan).threads, (smem), st, args);  \
-                              else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, false, false>), grid, (plan).threads, (smem), st, args); }         \
-        }                                                                                                                        \
+// Rows that are not staged, with element loads.
+#define TPB_ELEMENT_LAUNCH(KERNEL, T, plan, grid, smem, st, args)                                                          \
+    do {                                                                                                                   \
+        if ((plan).warp) {                                                                                                 \
+            if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, false, true>), grid, (plan).threads, (smem), st, args);  \
+            else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, false, true>), grid, (plan).threads, (smem), st, args);                 \
+        } else {                                                                                                           \
+            if ((plan).nv == 1) TPB_LAUNCH(#KERNEL, (KERNEL<T, 1, false, false>), grid, (plan).threads, (smem), st, args); \
+            else TPB_LAUNCH(#KERNEL, (KERNEL<T, 2, false, false>), grid, (plan).threads, (smem), st, args);                \
+        }                                                                                                                  \
     } while (0)
 
 // shared memory for the kept elements of the CTA's rows, where rows are no whole blocks of the generator
@@ -776,7 +773,10 @@ int forward_run(const ForwardArgs<T>& k, cudaStream_t st) {
     }
     const RowPlan p = plan_rows(k.width, vec);
     const dim3 grid((unsigned)(p.warp ? ceil_div(k.rows, p.threads / 32) : k.rows));
-    TPB_BLOCK_LAUNCH(block_forward_kernel, T, p, grid, mask_bytes(p, k.width, k.drop), st, k);
+    // aligned rows are short ones or longer than the staged kernel takes
+    if (vec && p.warp) TPB_LAUNCH("block_forward_kernel", (block_forward_kernel<T, 1, true, true>), grid, p.threads, 0, st, k);
+    else if (vec) TPB_LAUNCH("block_forward_kernel", (block_forward_kernel<T, 2, true, false>), grid, p.threads, 0, st, k);
+    else TPB_ELEMENT_LAUNCH(block_forward_kernel, T, p, grid, mask_bytes(p, k.width, k.drop), st, k);
     return TPB200_OK;
 }
 
@@ -797,7 +797,17 @@ int backward_run(const BackwardArgs<T>& k, T* dpost, T* dnext, long long gate_gr
         if (rc != TPB200_OK) return rc;
         TPB_LAUNCH("block_backward_staged_kernel", kernel, dim3((unsigned)k.workers), threads, smem, st, k);
     } else {
-        TPB_BLOCK_LAUNCH(block_backward_kernel, T, p, grid, mask_bytes(p, k.width, k.drop), st, k);
+        // aligned rows are longer than the staged kernel takes: more than 8192 elements, or a float32 row whose stages do not fit
+        static_assert(sizeof(T) == 4 || 1024 * ((kStages * kStageArrays + 2) * 8 * sizeof(T) + 32) <= 226 * 1024, "16-bit rows of 8192 elements are staged");
+        auto kernel = block_backward_kernel<T, 2, true, false>;
+        if (!vec) {
+            TPB_ELEMENT_LAUNCH(block_backward_kernel, T, p, grid, mask_bytes(p, k.width, k.drop), st, k);
+        } else {
+            if constexpr (sizeof(T) == 4) {
+                if (p.nv == 1) kernel = block_backward_kernel<T, 1, true, false>;
+            }
+            TPB_LAUNCH("block_backward_kernel", kernel, grid, p.threads, 0, st, k);
+        }
     }
     const bool sum_gate = k.gate.p && !k.gate_rows && k.groups_per_worker == 0;
     if (!dpost && !dnext && !sum_gate) return TPB200_OK;

@@ -233,39 +233,6 @@ __device__ __forceinline__ uint4 grad_vector(const uint4& raw, const RowGrad& g,
     return Elem<T>::pack(v);
 }
 
-template <class T>
-__device__ __forceinline__ void sweep_grad(const T* p, T* o, int len, const RowGrad& g) {
-    constexpr int N = Elem<T>::N;
-    const int tid = threadIdx.x, nthr = blockDim.x;
-    if ((((uintptr_t)p ^ (uintptr_t)o) & 15) == 0) {
-        const Span<T> sp(p, len);
-        for (int i = tid; i < sp.nvec; i += nthr) {
-            const int j0 = sp.head + i * N;
-            float v[N];
-            Elem<T>::unpack(ld_once16(p + j0), v);
-#pragma unroll
-            for (int c = 0; c < N; ++c) v[c] = grad_at(v[c], j0 + c, g);
-            st_out16(o + j0, Elem<T>::pack(v));
-        }
-        if (tid < sp.head) *TPB_CK(&o[tid]) = Elem<T>::put(grad_at(Elem<T>::get(*TPB_CK(&p[tid])), tid, g));
-        if (tid < sp.tail) {
-            const int j = len - 1 - tid;
-            *TPB_CK(&o[j]) = Elem<T>::put(grad_at(Elem<T>::get(*TPB_CK(&p[j])), j, g));
-        }
-    } else {
-        for (int j = tid; j < len; j += nthr) *TPB_CK(&o[j]) = Elem<T>::put(grad_at(Elem<T>::get(*TPB_CK(&p[j])), j, g));
-    }
-}
-
-template <class T>
-__device__ __forceinline__ void sweep_zero(T* o, int len) {
-    const Span<T> sp(o, len);
-    const int tid = threadIdx.x, nthr = blockDim.x;
-    for (int i = tid; i < sp.nvec; i += nthr) st_out16(o + sp.head + (size_t)i * Elem<T>::N, make_uint4(0, 0, 0, 0));
-    if (tid < sp.head) *TPB_CK(&o[tid]) = Elem<T>::put(0.0f);
-    if (tid < sp.tail) *TPB_CK(&o[len - 1 - tid]) = Elem<T>::put(0.0f);
-}
-
 // ---------------------------------------------------------------- log-probabilities ----------
 // The range of rows that belong to a sequence (all of them without offsets).
 struct RowLimits {
