@@ -828,7 +828,14 @@ int check_block(const char* what, int dtype, int64_t outer, int64_t inner, int64
     return TPB200_OK;
 }
 
-// groups of rows that share a row of the gate, by the gate's kind; 0: an unknown kind
+// Rows of no elements have no mean square: their rstd is NaN (all bits set).
+inline int empty_rows(long long rows, float* rstd_a, float* rstd_b, cudaStream_t st) {
+    for (float* p : {rstd_a, rstd_b})
+        if (rows > 0 && p) TPB_CUDA_OK(cudaMemsetAsync(p, 0xff, (size_t)rows * sizeof(float), st));
+    return TPB200_OK;
+}
+
+// groups of rows that share a row of the gate, by the gate's kind
 inline long long gate_groups_of(int kind, int64_t outer) { return kind == TPB200_GATE_SEQUENCE ? outer : 1; }
 
 struct BlockPointers { float *post, *next, *gate; size_t bytes; };
@@ -918,7 +925,7 @@ extern "C" int tpb200_rms_norm(const void* x, int dtype, int64_t outer, int64_t 
     const int rc = check_block("rms_norm", dtype, outer, inner, width);
     if (rc != TPB200_OK) return rc;
     if (!(eps >= 0.0)) return fail(TPB200_ERR_INVALID, "rms_norm: eps must not be negative");
-    if (outer * inner * width == 0) return TPB200_OK;
+    if (outer * inner * width == 0) return empty_rows(outer * inner, rstd, nullptr, (cudaStream_t)stream);
     if (!x || !strides || !weight || !y || !rstd) return fail(TPB200_ERR_INVALID, "rms_norm: NULL pointer argument");
     cudaStream_t st = (cudaStream_t)stream;
     [[maybe_unused]] const int64_t e = dtype_bytes(dtype), n = outer * inner;
@@ -939,7 +946,8 @@ extern "C" int tpb200_block_residual(const void* x, const int64_t* x_strides, co
     if (!(eps >= 0.0)) return fail(TPB200_ERR_INVALID, "block_residual: eps must not be negative");
     DropSpec drop;
     if (!make_drop(p, seed, offset, &drop)) return fail(TPB200_ERR_INVALID, "block_residual: p must lie in [0, 1]");
-    if (outer * inner * width == 0) return TPB200_OK;
+    // (weights of no elements may be NULL: the outputs say which norms there are)
+    if (outer * inner * width == 0) return empty_rows(outer * inner, rstd_post, rstd_next, (cudaStream_t)stream);
     if (!x || !h || !x_out || !x_strides || !h_strides || (gate && !gate_strides) || (post_weight && !rstd_post) || (next_weight && (!y || !rstd_next)))
         return fail(TPB200_ERR_INVALID, "block_residual: NULL pointer argument");
     cudaStream_t st = (cudaStream_t)stream;

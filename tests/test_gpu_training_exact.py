@@ -95,6 +95,20 @@ def test_x_in_place_of_x_out_as_a_view_and_without_a_next_norm(cuda, tpb, dtype)
         tpb.block_residual_backward(v["gx"], v["gy"], v["h"], None, rp, rp, v["post"], v["next"], v["gate"])
 
 
+@EACH
+def test_rows_of_no_elements(cuda, tpb, dtype):
+    """The mean square of nothing is NaN, and so is rstd: it is written, not left as it was."""
+    x, w = torch.empty(3, 5, 0, dtype=dtype, device=cuda), torch.empty(0, dtype=dtype, device=cuda)
+    y, rstd = tpb.rms_norm(x, w, out=(torch.empty_like(x), torch.full((3, 5), 7.0, device=cuda)))
+    assert y.shape == x.shape and bool(rstd.isnan().all())
+    out = (torch.empty_like(x), torch.empty_like(x), *(torch.full((3, 5), 7.0, device=cuda) for _ in range(2)))
+    _, _, rp, rn = tpb.block_residual(x, x, w, w, out=out)
+    assert bool(rp.isnan().all()) and bool(rn.isnan().all())
+    assert all(g is None or g.numel() == 0 for g in tpb.block_residual_backward(x, x, x, x, rp, rn, w, w))
+    none = torch.empty(0, 8, dtype=dtype, device=cuda)
+    assert tpb.rms_norm(none, torch.ones(8, dtype=dtype, device=cuda))[1].shape == (0,)
+
+
 # ------------------------------------------------------------------------------------ objectives on logits
 
 def exact_rows(x, labels):
