@@ -362,7 +362,8 @@ size_t tpb200_preference_loss_workspace_bytes(int64_t outer, int64_t inner, int6
 /* Dropout from a counter-based generator (Philox 4x32-10): element i in row-major order is kept iff its 16
  * bits of the block with counter (i / 8, offset) and key `seed` reach p in units of 2^-16 (rounded); kept
  * elements are multiplied by 1 / (1 - p), with the p that was used, dropped ones are 0.  No mask is stored:
- * the backward pass is the same call on the gradient.  0 <= p <= 1.
+ * the backward pass is the same call on the gradient.  0 <= p <= 1.  seed and offset are values of the call: a
+ * captured graph holds them, and every replay drops the same elements.
  */
 int tpb200_dropout(const void* x, int dtype, int64_t outer, int64_t inner, int64_t width, const int64_t* strides,
                    double p, uint64_t seed, uint64_t offset, void* y, void* stream);

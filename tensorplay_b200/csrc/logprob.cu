@@ -286,7 +286,9 @@ __device__ __forceinline__ void fetch_token(const PolicyTerms& t, long long a, l
     if (t.ref.p) copy_async4(&k->ref, t.ref.p + a * t.ref.s0 + b * t.ref.s1);
 }
 
-// The row's outputs and its coefficient d loss / d logp:
+// The row's outputs and its coefficient d loss / d logp, in float32 from differences of float64 log-probabilities: the outputs
+// are float32, each is a few roundings of 2^-24 off (measured against 64 bits: ratio 6e-8, kl 2e-7 of their norms), and
+// float64 exponentials by one thread would lengthen every row.  The sum over the rows is float64.
 //   l = -min(r A, clip(r, 1 - low, 1 + high) A) + kl_coef (e^d - d - 1),  r = e^(logp - old), d = ref - logp
 //   dl / d logp = -r A (where the unclipped branch is the smaller one) + kl_coef (1 - e^d)
 struct PolicyRow { float ratio, kl, coef; double part; };
@@ -394,9 +396,9 @@ __device__ __forceinline__ void leave_out(uint4 (&raw)[VECS], int e) {
 // Running sum of 2^(c x - E) of one thread over a row, two vectors at a time, against a reference that is fixed
 // after the first step, the maximum of what the warp has met there: no maximum and no rescaling per element.  A step
 // whose sum is not below 2 -- values well above the reference, infinities, NaN, far rows (their E is NaN) -- is done
-// again the careful way, which raises the reference.  (A running maximum took 25 instructions per element in all, this
-// 14.)  The exponent is kRest x + (kStep x - E): two roundings, of 2^-22 at most for float32 below 8 and |x| below 1500, the
-// first of them none for a 16-bit type.
+// again the careful way, which raises the reference.  The exponent is kRest x + (kStep x - E): two roundings, of 2^-22 at
+// most below 8 octaves and |x| of 1500, the first of them none for a 16-bit type.  Nine thread instructions per
+// element in all ([2048,50016] bf16, counted by the profiler), of which one is ex2 on a pipe of 16 a cycle.
 template <class T>
 struct FixedSum {
     static constexpr int N = Elem<T>::N;
@@ -572,13 +574,14 @@ constexpr int kRowCluster = 8;
 // row's 16-byte vectors.  The first sweep sums, the CTAs' (sum, reference) pairs cross the cluster through
 // distributed shared memory, and the second sweep writes the gradient; it reads the row again, from L2,
 // because C is chosen so that the rows in flight take half of it (row_shape), and because loads and stores say
-// what may be evicted.  Bytes from and to memory are then near one read and one write.  What bounds it: two
-// ex2 per element, 16 a cycle on an SM (249 of 360 us on [4096,151936] bf16 with 90 % of the rows counted), nine
-// instructions per element, and the second read through L2; 2048 threads on an SM hide their latencies.
-// Measured, of one read and one write: [4096,50016] bf16 4.97 TB/s (C = 1), [1024,151936] bf16 4.46 (C = 3),
-// f32 4.83 (C = 6); with two CTAs of 512 on an SM instead of four 4.0, 4.0 and 4.3; in separate kernels for
-// sum and gradient 3.8 and 3.8.  Keeping the row in shared memory instead (a ring of bulk copies, persistent CTAs)
-// left 16 to 26 warps on an SM to hide the latencies and was slower: 4.6, 4.0 and 3.2.
+// what may be evicted.  Bytes from and to memory are then near one read and one write.  What bounds the losses: two
+// ex2 per element, 16 a cycle on an SM (249 of 360 us on [4096,151936] bf16 with 90 % of the rows counted; the pipe is 62 %
+// busy, the issue slots 56 %), and the second read through L2; 2048 threads on an SM hide their latencies.
+// Measured, of one read and one write: [4096,50016] bf16 4.90 TB/s (C = 1), [1024,151936] bf16 4.38 (C = 3),
+// f32 4.59 (C = 6); the backward call, most rows by lse: 6.11, 5.98 (C = 3).  An earlier form, without the exact sums and
+// at 4.97, 4.46 and 4.83, was the base of these comparisons: two CTAs of 512 on an SM instead of four 4.0, 4.0
+// and 4.3; separate kernels for sum and gradient 3.8 and 3.8; the row kept in shared memory (a ring of bulk copies,
+// persistent CTAs), which left 16 to 26 warps on an SM to hide the latencies, 4.6, 4.0 and 3.2.
 enum Mode { kScores, kPolicy, kBackward };
 template <class T, int MODE>
 __global__ void __launch_bounds__(kRowThreads, kRowCtas)
@@ -854,8 +857,10 @@ inline PerToken<float> per_token(const float* p, const int64_t* strides) {
 // Threads of a CTA and CTAs per row.  Short rows get as many threads as they have pairs of vectors.  More than one
 // CTA per row: with a second sweep, so that the rows in flight (four CTAs on every SM) take at most 60 MB, half
 // of L2; and while all CTAs fit the GPU at once and a CTA still has a vector per thread.  Policy loss on [1024,151936],
-// bf16, C = 1, 2, 3, 4, 6: 4.10, 4.38, 4.46, 4.33, 3.94 TB/s; f32: 4.12, 4.20, 4.44, 4.44, 4.83.  Scores of [256,151936] f32,
-// C = 1, 2 (512 CTAs of 592), 3, 4: 34.6, 28.7, 34.5, 32.2 us; of [1,151936] bf16, C = 1, 4, 8: 11.0, 6.1, 4.8 us.
+// bf16, C = 1, 2, 3, 4, 6: 4.11, 4.30, 4.36, 4.23, 3.85 TB/s; f32: 4.13, 4.18, 4.37, 4.34, 4.59; on [4096,50016] bf16, C = 1, 2:
+// 4.90, 4.11.  Scores of [256,151936] f32, C = 1, 2 (512 CTAs of 592), 3, 4: 34.6, 29.0, 36.8, 34.5 us; of [1,151936] bf16,
+// C = 1, 4, 8: 12.6, 7.4, 6.0 us.  The backward call goes by the rule of two sweeps, though it mostly needs one:
+// [1024,151936] bf16, C = 1, 2, 3, 4: 107, 106, 105, 104 us.
 struct RowShape { int threads, C; };
 inline RowShape row_shape(int64_t rows, int64_t vocab, int64_t elem, bool twice) {
     const int64_t vectors = vocab * elem / 16, room = 4LL * sm_count();
@@ -864,7 +869,7 @@ inline RowShape row_shape(int64_t rows, int64_t vocab, int64_t elem, bool twice)
     int64_t C = 1;
     if (twice) C = std::min<int64_t>(kRowCluster, ceil_div(std::min(rows, room) * vocab * elem, 60LL << 20));
     while (C < kRowCluster && rows * (C + 1) <= room && vectors >= (C + 1) * kRowThreads) ++C;
-    int forced = 0;      // experiment and test switch: that many CTAs per row
+    int forced = 0;      // experiment and test switch: that many CTAs per row (tests run every kernel at 1 to 8)
     if (env_int("TPB200_ROW_CTAS", &forced) && forced >= 1 && forced <= kRowCluster) C = forced;
     if (rows * C > 0x7fffffffLL) C = 1;
     s.C = (int)C;

@@ -16,6 +16,11 @@ more and rounded once.  Rows are the last dim, which must have unit stride; the 
 strides as long as all but the last of them collapse to one.  Results are contiguous, and a gradient has
 the type of what it is the gradient of.  The functions only enqueue on the current stream; scratch memory
 comes from torch's allocator on every call, so that calls on other streams and captured graphs share none.
+
+No function records an autograd graph, whatever its inputs require: the gradients come from the *_backward functions
+and from the losses themselves (wrap them in a torch.autograd.Function to use them in one).  `seed` and `offset` of
+a dropout are numbers of the call: a captured graph holds them, and every replay drops the same elements.
+To drop others, capture once per offset, or call dropout outside of the graph.
 """
 from __future__ import annotations
 
@@ -221,7 +226,9 @@ def token_logprobs(logits, labels, *, out=None):
 
 def token_logprobs_backward(grad_logp, logits, labels, lse, *, out=None):
     """Gradient of token_logprobs' logp: grad_logp * (one at the label - softmax(logits)), in the logits'
-    type.  `grad_logp` (float32) broadcasts to the tokens; `lse` is the forward call's.  `out=(grad_logits,)`."""
+    type.  `grad_logp` (float32) broadcasts to the tokens; `lse` is the forward call's.  Rows whose float32 lse
+    does not hold the digits (|lse| of 32 and more, a token with half of the probability) are summed again.
+    `out=(grad_logits,)`."""
     what = "token_logprobs_backward"
     rows, lab = _logits(logits, labels, what)
     grad = _token(grad_logp, logits, torch.float32, what, "grad_logp", broadcast=True)
@@ -420,6 +427,7 @@ def block_residual(x, h, post_weight=None, next_weight=None, gate=None, *, scale
         y = rms_norm(x_out) * next_weight                 (None without next_weight)
 
     `gate`: [width], one row per sequence ([..., 1, width]), or x.shape.  y goes by x_out before it is rounded.
+    seed and offset as in dropout (a captured graph drops the same elements on every replay).
     Returns (x_out, y, rstd_post, rstd_next); the last two (float32 per row, None where there is no norm)
     are for the backward pass.  `out`: these four."""
     what = "block_residual"
@@ -515,7 +523,8 @@ def dropout(x, p, seed, offset=0, *, out=None):
     """x with every element dropped with probability p (in units of 2^-16, rounded) and the kept ones
     multiplied by 1 / (1 - p).  The choice is a function of the element's position in row-major order, of
     `seed` and of `offset` (both 0 .. 2^64 - 1) alone: no mask is stored, and the same call on the gradient
-    is the backward pass.  Use another offset for every call of a step.  `out=(y,)`."""
+    is the backward pass.  Use another offset for every call of a step; a captured graph keeps the one it was
+    captured with, and drops the same elements on every replay.  `out=(y,)`."""
     return _dropout(x, p, seed, offset, out, "dropout")
 
 

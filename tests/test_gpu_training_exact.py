@@ -1,6 +1,9 @@
 """GPU tests of what the training operators keep of their 64-bit formulas where digits are easily lost, and of
 calls that are rarely made.  Oracles in 64 bits; every bound is derived where it stands (u = eps / 2 is one
 rounding of the output)."""
+import os
+import subprocess
+import sys
 import threading
 
 import pytest
@@ -379,3 +382,74 @@ def test_two_host_threads_with_different_widths(cuda, tpb, dtype):
     assert not errors, errors[0]
     for a, b in zip(want, got):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+# ------------------------------------------------------------------------------------ how they are called
+
+def test_captured_where_the_data_decides(cuda, tpb):
+    """One graph over rows that the backward call takes by lse in one replay and sums again in the next, over rows that
+    change between near and far, and over the residual path by x; equal to eager calls every time."""
+    vocab, n = 20011, 24
+    x = torch.zeros(n, vocab, dtype=torch.bfloat16, device=cuda)
+    lab, coef = torch.zeros(n, dtype=torch.int64, device=cuda), torch.ones(n, device=cuda)
+    v = block_inputs(cuda, (2, 9, 640), torch.bfloat16, "sequence", 82)
+
+    def run():
+        logp, lse = tpb.token_logprobs(x, lab)
+        g = tpb.token_logprobs_backward(coef, x, lab, lse)
+        x_out, y, rp, rn = tpb.block_residual(v["x"], v["h"], v["post"], v["next"], v["gate"], p=0.1, seed=1)
+        return [logp, lse, g, *tpb.policy_loss(x, lab, logp - 0.1, coef, coef, logp + 0.1, kl_coef=0.1), x_out, y,
+                *tpb.block_residual_backward(v["gx"], v["gy"], v["h"], None, rp, rn, v["post"], v["next"], v["gate"], x=v["x"], p=0.1, seed=1)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        kept = run()
+    sure, at = confident(cuda, torch.bfloat16, vocab, 5)
+    far, far_at = far_rows(cuda, torch.bfloat16, vocab)
+    for rows, labels in ((logits_of(cuda, (n, vocab), torch.bfloat16, 1), labels_of(cuda, (n,), vocab, 2, 0.2)), (sure[:n], at[:n]),
+                         (torch.cat([far, sure])[:n], torch.cat([far_at, at])[:n]), (logits_of(cuda, (n, vocab), torch.bfloat16, 3), labels_of(cuda, (n,), vocab, 4))):
+        x.copy_(rows)
+        lab.copy_(labels)
+        v["h"].copy_(logits_of(cuda, v["h"].shape, torch.bfloat16, int(labels[0]) + 7))
+        graph.replay()
+        eager = run()
+        torch.cuda.synchronize()
+        for a, b in zip(kept, eager):
+            assert a is None or torch.equal(a, b)
+
+
+def test_a_captured_dropout_drops_the_same_elements(cuda, tpb):
+    """As documented: seed and offset are numbers of the call, so that a graph repeats the choice it was captured with."""
+    x = torch.ones(1000, device=cuda)
+    tpb.dropout(x, 0.5, 3, 4)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = tpb.dropout(x, 0.5, 3, 4)
+    for scale in (1.0, 2.0):
+        x.fill_(scale)
+        graph.replay()
+        assert torch.equal(y, tpb.dropout(x, 0.5, 3, 4)) and not torch.equal(y, tpb.dropout(x, 0.5, 3, 5))
+
+
+def test_no_function_records_a_graph(cuda, tpb):
+    """As documented: inputs that require gradients are read, and nothing is recorded."""
+    x = torch.randn(4, 8, device=cuda, requires_grad=True)
+    lab, one, w = labels_of(cuda, (4,), 8, 2), torch.ones(4, device=cuda), torch.ones(8, device=cuda, requires_grad=True)
+    for t in (*tpb.token_logprobs(x, lab), *tpb.policy_loss(x, lab, one, one, one), *tpb.rms_norm(x, w), *tpb.block_residual(x, x.detach(), w, w), tpb.dropout(x, 0.5, 1)):
+        assert not t.requires_grad
+
+
+def test_under_the_range_checker(cuda):
+    """The tests of this file with every global access compared with the ranges of its call."""
+    from tensorplay_b200 import _lib
+    if _lib.CHECKED:
+        pytest.skip("already running under the checked build")
+    r = subprocess.run([sys.executable, "-m", "pytest", os.path.join("tests", "test_gpu_training_exact.py"), "-x", "-q", "-m", "gpu", "-p", "no:cacheprovider",
+                        "-k", "not host_threads and not captured and not one_side and not of_their_own"],
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), env=dict(os.environ, TPB200_CHECKED="1"), capture_output=True, text=True, timeout=1500)
+    assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-2000:]
