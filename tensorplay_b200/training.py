@@ -150,7 +150,12 @@ def _ptr(t):
 def _outputs(what, like, out, specs):
     """New contiguous outputs, or the ones of `out` after a check; specs: (shape, dtype) or None each."""
     if out is None:
-        return [None if s is None else _new(s[0], s[1], like) for s in specs]
+        outs, last = [], None
+        for s in specs:
+            # the same spec again: empty_like takes half the time of new_empty
+            outs.append(None if s is None else torch.empty_like(outs[-1]) if s is last else _new(s[0], s[1], like))
+            last = s
+        return outs
     device = like.device
     if not isinstance(out, (tuple, list)) or len(out) != len(specs):
         raise ValueError(f"{what}: out must hold {len(specs)} tensors")
