@@ -14,7 +14,7 @@
 //     distance of the logits, and a reward adds that up over its sequence.  (With c a float32 rewards of [3001,151936]
 //     were 1.2e-6 of themselves off.)  The gradient, whose entries stand by themselves, takes one multiply-add
 //     with the float32 c.
-//   * Where |m| >= 2^12 (rows of a type's lowest value are such rows) x - m is formed first.
+//   * Where |m| >= 2^15 (rows of a type's lowest value are such rows) x - m is formed first.
 //   * s is kept in float32, a few hundred terms per thread at most, and joined by trees;
 //   * the per-row scalars (log s, g, logp, differences of log-probabilities) are formed in float64 from an
 //     exponent and a mantissa; the gradient at the token itself is coef * (1 - p_y).
@@ -41,7 +41,7 @@ constexpr float kLow = (1.4426950408889634 - (double)kLog2e) / 1.442695040888963
 // ex2.approx is low by this on average over an octave of negative arguments (2^22 of them measured, each off by at most
 // 1.5e-7); a sum of many terms is low by as much, always to the same side
 constexpr double kExLow = 5.0e-8;
-constexpr float kFar = 4096.0f;          // |reference| from which x - m is formed first
+constexpr float kFar = 32768.0f;         // |reference| from which x - m is formed first: log-probabilities of [2048,50016] bf16 44 us, there 85
 constexpr float kAbove = 6.0f;           // octaves of E above the reference, so that no argument of ex2 is above 1
 
 __device__ __forceinline__ float ex2(float x) {
@@ -397,7 +397,7 @@ __device__ __forceinline__ void leave_out(uint4 (&raw)[VECS], int e) {
 // after the first step, the maximum of what the warp has met there: no maximum and no rescaling per element.  A step
 // whose sum is not below 2 -- values well above the reference, infinities, NaN, far rows (their E is NaN) -- is done
 // again the careful way, which raises the reference.  The exponent is kRest x + (kStep x - E): two roundings, of 2^-22 at
-// most below 8 octaves and |x| of 1500, the first of them none for a 16-bit type.  Nine thread instructions per
+// most below 8 octaves, the first of them none for a 16-bit type and up to 2^-32 |x| for a float32 above 1500.  Nine thread instructions per
 // element in all ([2048,50016] bf16, counted by the profiler), of which one is ex2 on a pipe of 16 a cycle.
 template <class T>
 struct FixedSum {
